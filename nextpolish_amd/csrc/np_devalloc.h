@@ -1,10 +1,10 @@
 // Device allocations of both libraries go through here.
 //
-// Default (round 6): a caching allocator in front of hipMalloc / hipFree (BlockCache below).  Why: on this runtime every hipFree first
-// waits for EVERY stream of the process (hip::Stream::SyncAllStreams; profiles/r5_fault_hunt.txt section 3 measured it), and a drop-in
-// call or a tile allocates and frees ~110 buffers -- a long-lived worker (the reference's caller: one process, contig after contig,
-// source/lib/nextpolish1.py:181-189,219-224) made ~65 000 such device-wide waits per test-suite run, and the one-process suite stopped
-// inside one of them in rounds 4 and 5.  With the cache a released buffer goes to a per-device free list and the
+// A caching allocator in front of hipMalloc / hipFree (BlockCache below).  Why: on this runtime hipFree waits for work of OTHER streams
+// (measured: a buffer that a 300 ms kernel of another non-blocking stream was writing took 300.3 ms to free, profiles/r5_fault_hunt.txt
+// section 3), and a drop-in call or a tile allocates and frees ~110 buffers -- a long-lived worker (the reference's caller: one process,
+// contig after contig, source/lib/nextpolish1.py:181-189,219-224) made ~65 000 such waits per run of the test suite, and the one-process
+// suite was seen to stop inside a release.  With the cache a released buffer goes to a per-device free list and the
 // next request of a similar size takes it from there: no runtime call on either side in steady state.  The guarantee hipFree gave --
 // nothing in flight still touches the block when somebody else gets it -- is kept without waiting: at release time every stream either
 // library created (stream_create below keeps the registry) is asked with hipStreamQuery; for each one that is busy an event is
@@ -136,13 +136,12 @@ inline void busy_streams(int dev, std::vector<hipStream_t>* out) {
     for (hipStream_t q : all) if (hipStreamQuery(q) == hipErrorNotReady) out->push_back(q);
 }
 
-// Before memory really goes back to the runtime.  hipFree and hipHostFree first wait for every stream of the process, and they wait the
-// fragile way: HostQueue::finish(cpu_wait = true) -> Command::awaitCompletion(), i.e. the calling thread sleeps on a condition variable until
-// the runtime's signal-handler thread marks the stream's last command complete -- and that wake-up sometimes never comes (round 6: three
-// stops of the test process, all inside hipFree, every queue idle and hipStreamQuery answering "ready" for every stream; DESIGN.md section
-// 12, profiles/r6_hang_hunt.txt).  hipStreamSynchronize waits on the hardware signal itself and, once it returns, the stream has no "last
-// command" left for hipFree to wait for.  So every stream of the registry and the null stream are synchronised that way first, under one
-// lock so that two releasing threads do not interleave; hipFree then finds nothing to wait for.
+// Before memory really goes back to the runtime.  hipFree and hipHostFree wait for work in flight on every stream, and a release was seen
+// not to return at all: three stops of the test process inside this project's own release path (DevBuf::ensure, np1_batch_free; the last
+// one in BlockCache::put, which with the cache off calls hipFree and nothing else), while hipStreamQuery answered "ready" for every stream
+// of the process (profiles/r6_hang_hunt.txt).  hipStreamSynchronize was not seen to stop.  So every stream of the registry and the null
+// stream are synchronised with it first, under one lock so that two releasing threads do not interleave: the release itself then has no
+// work in flight to wait for.
 inline std::mutex& raw_free_mutex() { static std::mutex* m = new std::mutex(); return *m; }
 inline void quiesce() {
     std::vector<hipStream_t> all;
@@ -355,8 +354,7 @@ inline hipError_t host_free(void* p) {
     return host_cache().put(p);
 }
 // What a stopped process can say about itself (tests/conftest.py's watchdog calls np1_diag_report / np2_diag_report from a helper thread):
-// every stream of the registry with hipStreamQuery's answer, and the cache counters.  A stream that answers "ready" while another thread sits
-// in a runtime wait is a wake-up the runtime lost; one that answers "not ready" on an idle GPU is work the runtime never finished.
+// every stream of the registry with hipStreamQuery's answer, and the cache counters: whether the stopped thread still has work to wait for.
 inline void report(int fd, const char* who) {
     std::vector<std::pair<hipStream_t, int>> all;
     {

@@ -199,9 +199,8 @@ inline hipError_t d2h(void* dst, const void* src, size_t bytes, hipStream_t q) {
     return err;
 }
 
-// the synchronous forms: on the null stream, complete on return.  (Not hipMemcpy: the synchronous API waits through
-// Command::awaitCompletion, the wake-up by the runtime's handler thread that hipFree was seen to lose -- np_devalloc.h, quiesce;
-// hipMemcpyAsync + hipStreamSynchronize waits on the hardware signal.)
+// the synchronous forms: on the null stream, complete on return.  (hipMemcpyAsync + hipStreamSynchronize, not hipMemcpy: every wait of the
+// libraries is one of the stream waits, which were never seen to stop -- np_devalloc.h, quiesce.)
 inline hipError_t h2d_sync(void* dst, const void* src, size_t bytes) {
     if (!bytes) return hipSuccess;
     const hipError_t e = h2d(dst, src, bytes, nullptr);

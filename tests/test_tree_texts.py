@@ -1,0 +1,36 @@
+"""What the sources, documents, profiles and tools of the tree may hold (CPU)."""
+import os
+import re
+
+from conftest import ROOT
+
+PARTS = ("nextpolish_amd", "include", "tests", "tools", "oracle", "docs", "profiles",
+         "DESIGN.md", "INTEGRATION.md", "README.md", "bench.py", "__graft_entry__.py", "pytest.ini")
+KINDS = (".py", ".sh", ".c", ".cpp", ".h", ".hip", ".md", ".txt", ".ini", "Makefile")
+
+
+def texts():
+    """(path relative to the root, text) of every source, script, document and profile; built files, fixtures and this file are left out."""
+    for part in PARTS:
+        top = os.path.join(ROOT, part)
+        for d, dirs, names in os.walk(top) if os.path.isdir(top) else [(ROOT, [], [part])]:
+            dirs[:] = [x for x in dirs if x not in ("__pycache__", "build", "lib", "bin", "_ref", "golden")]
+            for n in sorted(names):
+                p = os.path.join(d, n)
+                if n.endswith(KINDS) and p != os.path.abspath(__file__):
+                    with open(p, errors="replace") as f:
+                        yield os.path.relpath(p, ROOT), f.read()
+
+
+def test_no_text_reads_offsets_of_an_installed_library():
+    # An offset into a library that was not built here is only ever part of an unannotated back trace, "lib.so.N(+0x...)[0x...]": a text that
+    # gives one a meaning rests on the library's code.
+    trace = re.compile(r"\S+\.so\.\d+\(\S*\+0x[0-9a-f]+\)\[0x[0-9a-f]+\]")
+    offset = re.compile(r"\+0x[0-9a-f]{4,}")
+    bad = []
+    for path, text in texts():
+        for k, line in enumerate(text.splitlines(), 1):
+            rest = re.sub(r"\S+/nextpolish_amd/lib/\S+", "", trace.sub("", line))      # (offsets into the project's own libraries are its own)
+            if offset.search(rest):
+                bad.append("%s:%d" % (path, k))
+    assert not bad, bad
