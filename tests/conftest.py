@@ -14,7 +14,7 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a real MI355X (run with -m gpu on the GPU box)")
     # a fatal signal inside native code (ours, the HIP runtime's) must leave enough behind to be read afterwards
     # (pytest's own faulthandler plugin prints them on stderr; the libraries add the native frames of the aborting thread and the exception
-    # behind a std::terminate when NP_ABORT_TRACE is set: csrc/np_diag.cpp, DESIGN.md §12)
+    # behind a std::terminate when NP_ABORT_TRACE is set: csrc/np_diag.cpp)
     d = os.path.join(ROOT, "gpurun_out")
     os.makedirs(d, exist_ok=True)
     os.environ.setdefault("NP_ABORT_TRACE", os.path.join(d, "abort_%d.txt" % os.getpid()))
@@ -24,16 +24,16 @@ def pytest_configure(config):
 
 # ------------------------------------------------------------------------------------------------- a test that STOPS must say where
 #
-# Round 5 ended with the one-process GPU suite stopped inside one native call and nothing to read: pytest-timeout prints Python frames only.
+# pytest-timeout prints Python frames only; a test that stopped inside a native call needs more to be read afterwards.
 # This watchdog (a daemon thread of the test process) ends a test that has been running for NP_TEST_WATCHDOG_S seconds (default 300; the
 # longest test of the suite takes about two minutes; 0 switches it off) and leaves, in gpurun_out/hang_<pid>.txt and on stderr:
 #   1. the state and kernel wait channel of every thread (/proc/self/task/*), which tells a thread blocked inside a driver ioctl from one
 #      spinning or sleeping in user space;
-#   2. rocgdb attached to the process for a moment: every host thread's native stack, and the GPU side -- agents, queues, dispatches in
-#      flight and the waves still running, each with the kernel it belongs to;
+#   2. what the loaded libraries say about their streams (hipStreamQuery) and allocator caches;
 #   3. Python's frames of every thread (faulthandler);
 # then sends SIGABRT to the main thread, so csrc/np_diag.cpp prints the native frames of the blocked thread and of every other thread from
-# inside the process (the fallback when no debugger can attach), and the process ends with a core-dump status instead of hanging.
+# inside the process, and the process ends with a core-dump status instead of hanging.  Nothing is attached to the process and no other
+# program is started.
 _beat = {"t": 0.0, "name": None}
 
 
@@ -58,24 +58,6 @@ def _thread_states():
             row.append("syscall=?")
         out.append(" ".join(row))
     return "\n".join(out)
-
-
-def _debugger_dump(path):
-    gdb = "/opt/rocm/bin/rocgdb"
-    if not os.path.exists(gdb):
-        return "no rocgdb on this box\n"
-    cmds = ["set pagination off", "set confirm off", "set print thread-events off", "info agents", "info queues", "info dispatches",
-            "info threads", "thread apply all -q bt 40"]
-    argv = [gdb, "-q", "-batch", "-p", str(os.getpid())]
-    for c in cmds:
-        argv += ["-ex", c]
-    try:
-        with open(path + ".gdb", "wb") as f:
-            subprocess.run(argv, stdout=f, stderr=subprocess.STDOUT, timeout=240, stdin=subprocess.DEVNULL)
-    except Exception as e:      # noqa: BLE001 (whatever happens, the rest of the report must still be written)
-        return "rocgdb did not finish: %r\n" % (e,)
-    txt = open(path + ".gdb", "rb").read().decode("utf-8", "replace")
-    return txt if len(txt) < (4 << 20) else txt[: 3 << 20] + "\n[... cut ...]\n" + txt[-(1 << 20):]
 
 
 def _library_report(path):
@@ -128,8 +110,6 @@ def _watchdog(limit, outdir):
             say("\n[np watchdog] %s has been running for %.0f s (limit %d s): collecting the state of process %d\n" % (name, time.time() - t0, limit, os.getpid()))
             say("[np watchdog] threads (tid comm wchan state syscall):\n" + _thread_states() + "\n")
             say("[np watchdog] the libraries' streams and allocator caches:\n" + _library_report(path) + "\n")
-            say("[np watchdog] debugger:\n" + _debugger_dump(path) + "\n")
-            say("[np watchdog] threads after the debugger let go:\n" + _thread_states() + "\n")
             say("[np watchdog] Python frames:\n")
             faulthandler.dump_traceback(file=f, all_threads=True)
             faulthandler.dump_traceback(file=2, all_threads=True)
@@ -145,11 +125,6 @@ def _start_watchdog(outdir):
     if limit <= 0 or _beat.get("started"):
         return
     _beat["started"] = True
-    try:      # let a debugger that is our child attach (yama ptrace_scope 1 only admits ancestors otherwise)
-        import ctypes
-        ctypes.CDLL(None).prctl(0x59616D61, ctypes.c_ulong(-1 & 0xFFFFFFFFFFFFFFFF), 0, 0, 0)
-    except Exception:      # noqa: BLE001
-        pass
     import threading
     threading.Thread(target=_watchdog, args=(limit, outdir), name="np-watchdog", daemon=True).start()
 
