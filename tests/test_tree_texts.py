@@ -34,3 +34,22 @@ def test_no_text_reads_offsets_of_an_installed_library():
             if offset.search(rest):
                 bad.append("%s:%d" % (path, k))
     assert not bad, bad
+
+
+def test_every_tool_that_a_text_names_is_there():
+    # (a document may name a tool with or without its folder; "name*" stands for several)
+    named = re.compile(r"\b(?:tests/)?tools/([A-Za-z0-9_]+(?:/[A-Za-z0-9_]+)?\.(?:sh|py|hip|cpp))")
+    have = {os.path.relpath(os.path.join(d, n), os.path.join(ROOT, top))
+            for top in ("tests/tools", "tools") for d, _, names in os.walk(os.path.join(ROOT, top)) for n in names}
+    bad = sorted({(path, m) for path, text in texts() for m in named.findall(text) if m not in have})
+    assert not bad, bad
+
+
+def test_nothing_repeats_the_test_runner_or_a_test_until_it_fails():
+    bad = []
+    for path, text in texts():
+        if path.endswith(".sh") and re.search(r"^\s*for \w+ in \$\(seq", text, re.M) and "pytest" in text:
+            bad.append(path)
+        if path.endswith(".py") and re.search(r"parametrize\(.*os\.environ", text):
+            bad.append(path)
+    assert not bad, bad

@@ -20,7 +20,6 @@ PY
 python tools/rocprof_summary.py stats $O/ks/ks_results.db > $O/np2_kernel_stats_5mb.txt 2>&1; rm -rf $O/ks
 head -14 $O/np2_kernel_stats_5mb.txt | cut -c1-120
 NP2_TIMING=1 NP_HOST_THREADS=8 NP_IO_THREADS=8 timeout 120 python /tmp/np2case/run.py 2>&1 | grep -a "np2 poa" | tail -3
-NP2_POA_BIG_ONLY=1 NP2_TIMING=1 NP_HOST_THREADS=8 timeout 120 python /tmp/np2case/run.py 2>&1 | grep -a -E "np2 poa|pseudo" | tail -3
 timeout 600 python -m pytest tests/test_gpu_tiling.py -x -q -m gpu -p no:cacheprovider > $O/tiling_tests.log 2>&1; echo "tiling tests rc=$? $(tail -1 $O/tiling_tests.log)"
 timeout 300 python __graft_entry__.py smoke > $O/smoke.log 2>&1; echo "smoke rc=$?"; tail -6 $O/smoke.log
 for m in 32 34 64 66 98; do timeout 120 gpurun_in/r5_probe2 $m; done > $O/probe2_more.log 2>&1; grep -c "exit 0" $O/probe2_more.log; grep -a "KILLED\|fault" $O/probe2_more.log | head

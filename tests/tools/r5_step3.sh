@@ -1,10 +1,9 @@
 #!/bin/bash
-# Round 5, third GPU step: the pseudo-seed kernels after the reconvergence fix -- the probe, the long-read tests, the 5 Mb window's kernel stats
+# Round 5, third GPU step: the pseudo-seed kernels after the reconvergence fix -- the long-read tests, the 5 Mb window's kernel stats
 cd "$(dirname "$0")/../.."
 R=$PWD
 O=$R/gpurun_out/r5
 mkdir -p $O
-timeout 200 tests/tools/r5_poa_probe.sh 2>&1 | cut -c1-260
 timeout 300 python -m pytest tests/test_gpu_np2.py -x -q -m gpu -p no:cacheprovider > $O/np2_tests.log 2>&1; echo "np2 tests rc=$? $(tail -1 $O/np2_tests.log)"
 python tests/tools/np2_make_case.py /tmp/np2case 5 20 > /dev/null
 cat > /tmp/np2case/run.py <<PY
