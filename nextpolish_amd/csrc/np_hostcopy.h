@@ -1,7 +1,7 @@
 // Host <-> device copies of both libraries go through here.
 //
 // Why (round 5): on this runtime (ROCm 7.2) hipMemcpy / hipMemcpyAsync with PAGEABLE host memory is served three ways,
-// by size (tests/tools/r5_stale_pin_probe.hip `thresh` under AMD_LOG_LEVEL=4, profiles/r5_fault_hunt.txt):
+// by size (its own log, AMD_LOG_LEVEL=4: profiles/r5_fault_hunt.txt section 2):
 //   <= 1 MiB          staged through the runtime's own pinned buffer: the bytes are taken (H2D) while the call runs;
 //   1 MiB .. 32 MiB   the USER's pages are locked in place ("Locking to pool", a userptr registration with the kernel driver), the DMA engine
 //                     reads / writes them directly and the call RETURNS WITHOUT WAITING -- the copy is really asynchronous;

@@ -53,3 +53,13 @@ def test_nothing_repeats_the_test_runner_or_a_test_until_it_fails():
         if path.endswith(".py") and re.search(r"parametrize\(.*os\.environ", text):
             bad.append(path)
     assert not bad, bad
+
+
+def test_the_tools_hold_no_gpu_program_and_nothing_registers_memory_that_exists():
+    bad = []
+    for path, text in texts():
+        if path.startswith(("tests/tools", "tools")) and (path.endswith(".hip") or re.search(r"^[^#\n]*\bhipcc\b", text, re.M)):
+            bad.append(path)      # (GPU code is built by nextpolish_amd/csrc/Makefile only)
+        if path.endswith((".hip", ".cpp", ".h", ".c")) and re.search(r"\bhipHostRegister\s*\(", text):
+            bad.append(path)
+    assert not bad, bad

@@ -65,8 +65,8 @@ if has np2; then
 fi
 if has tile9; then
   { echo "# bench.py --workload c3_100mb_30x --steps 3, tile stage per 13 Mb batch: NP1_TILE=3 (k_tile3, default) vs NP1_TILE=9 (k_tile9)";
-    PROBE=0 TESTS=0 KINDS="3 9" bash tests/tools/r4_tile9_ab.sh 2>&1 | grep -E "bench tile|stage_ms|value";
+    TESTS=0 KINDS="3 9" bash tests/tools/r4_tile9_ab.sh 2>&1 | grep -E "bench tile|stage_ms|value";
     echo "# k_tile9 phase clocks (NP1_T9_PHASES=1; shader-clock cycles per wave)";
-    NP1_T9_PHASES=1 PROBE=0 TESTS=0 KINDS=9 bash tests/tools/r4_tile9_ab.sh > /dev/null 2>&1; grep "k_tile9 cycles" gpurun_out/r4_tile9/bench_tile9.err | tail -2; } > $O/r4_tile9_ab.txt
+    NP1_T9_PHASES=1 TESTS=0 KINDS=9 bash tests/tools/r4_tile9_ab.sh > /dev/null 2>&1; grep "k_tile9 cycles" gpurun_out/r4_tile9/bench_tile9.err | tail -2; } > $O/r4_tile9_ab.txt
 fi
 ls -la $O

@@ -5,10 +5,6 @@ cd "$(dirname "$0")/../.."
 OUT=gpurun_out/r4_tile9
 mkdir -p "$OUT"
 W=${1:-c3_100mb_30x}
-if [[ "${PROBE:-1}" == 1 ]]; then
-  /opt/rocm/bin/hipcc --offload-arch=gfx950 -I nextpolish_amd/csrc -o /tmp/np_probe tests/tools/efence_probe.hip > "$OUT/probe.log" 2>&1 && timeout 120 /tmp/np_probe fault >> "$OUT/probe.log" 2>&1
-  echo "probe rc=$?"; tail -25 "$OUT/probe.log"
-fi
 if [[ "${TESTS:-1}" == 1 ]]; then
   timeout 900 python -m pytest tests/test_gpu_score_chain.py tests/test_real_data.py -m gpu -x -q -p no:cacheprovider > "$OUT/tests.log" 2>&1
   echo "tests rc=$?"; tail -15 "$OUT/tests.log"
