@@ -32,10 +32,9 @@ struct DevBuf {
     int ensure(size_t bytes, double slack = 1.0) {
         if (bytes <= cap && p) return 0;
         if (p) { (void)npalloc::dev_free(p); p = nullptr; cap = 0; }
-        // No kernel reads past the bytes it was given (round 4: the wide staging loads and the chase window clamp at the logical end;
-        // NP_EFENCE=1 places every buffer against an unmapped page to prove it, np_devalloc.h).  The 64 KiB behind each buffer are
-        // defence in depth only; under NP_EFENCE there is no slack at all.
-        size_t want = npalloc::efence() ? bytes : (size_t)((double)bytes * slack) + 65536;
+        // No kernel reads past the bytes it was given: the wide staging loads and the chase window clamp at the logical end.  The 64 KiB
+        // behind each buffer are defence in depth only.
+        const size_t want = (size_t)((double)bytes * slack) + 65536;
         if (!hip_ok(npalloc::dev_malloc(&p, want), "hipMalloc")) { p = nullptr; return -1; }
         cap = want;
         return 0;

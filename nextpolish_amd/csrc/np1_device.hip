@@ -105,7 +105,7 @@ const char* np1_stage_name(int i) {
 }
 
 // Every uploaded array carries 64 bytes of pad: the kernels stage pools with 16-byte loads from 16-byte aligned addresses, which reach
-// up to 15 bytes past the last element (the pad is part of the allocation, not slack the allocator happens to leave: NP_EFENCE=1)
+// up to 15 bytes past the last element (the pad is part of the allocation, not slack the allocator happens to leave)
 static int upload(DevBuf& b, const void* src, size_t bytes, hipStream_t st) {
     if (b.ensure(bytes + 64) != 0) return -1;
     if (bytes) HIPCHK(npcopy::h2d(b.p, src, bytes, st));

@@ -56,7 +56,7 @@ struct DevBuf {
     bool ensure(size_t bytes) {
         if (bytes <= cap && p) return true;
         if (p) { (void)npalloc::dev_free(p); p = nullptr; cap = 0; }
-        const size_t want = npalloc::efence() ? bytes : bytes + bytes / 4 + 256;      // NP_EFENCE=1: the buffer ends where its mapping ends (np_devalloc.h)
+        const size_t want = bytes + bytes / 4 + 256;
         if (npalloc::dev_malloc(&p, want) != hipSuccess) { p = nullptr; return false; }
         cap = want;
         return true;

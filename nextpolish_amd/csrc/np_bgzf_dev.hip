@@ -51,7 +51,7 @@ struct DevInflater {
         if (*p) { if (host) (void)npalloc::host_free(*p); else (void)npalloc::dev_free(*p); }
         *p = nullptr;
         *cap = 0;
-        const size_t n = (!host && npalloc::efence()) ? want : want + want / 4 + (1u << 20);
+        const size_t n = want + want / 4 + (1u << 20);
         const hipError_t e = host ? npalloc::host_malloc(p, n, hipHostMallocPortable) : npalloc::dev_malloc(p, n);
         if (e != hipSuccess) { *p = nullptr; return false; }
         *cap = n;

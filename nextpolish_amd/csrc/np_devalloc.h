@@ -14,17 +14,11 @@
 // bound the largest idle blocks go back to the runtime, and when hipMalloc runs out of memory the cache is emptied and the request retried.
 // Whenever memory does go back to the runtime, every stream is synchronised with hipStreamSynchronize first (quiesce below, and why).
 //
-// NP_EFENCE=1 (debugging): every buffer is placed through the HIP virtual-memory API so that its LAST byte (rounded up to 16, the
-// widest vector access the kernels use) is the last mapped byte of its own address reservation, with an unmapped granule behind it.
-// A kernel that reads or writes past the end of a buffer then faults at the first such access, deterministically, instead of
-// touching whatever the allocator happened to place there (how the over-reads behind the round-3 abort were
-// found).  The mode costs one granule (2 MiB) of physical memory per buffer and a few hundred microseconds per allocation.
-//
 // NP_DEVPOISON=1 (debugging; or a hex byte, e.g. NP_DEVPOISON=ff): every new device buffer is filled with that byte (default a5) before it
 // is handed out.  hipMalloc hands a long-lived process the bytes of whatever it freed before -- a fresh process mostly sees zeros -- so a
 // kernel that reads memory nobody wrote behaves differently in the one-process test suite than in any single test; with the poison it
 // misbehaves the same way everywhere.  NP_DEVPOISON=2 also fills the work buffers of a short-read batch before
-// every run (what an earlier run left in a reused buffer is the other thing only a long-lived process has).  Works with and without NP_EFENCE.
+// every run (what an earlier run left in a reused buffer is the other thing only a long-lived process has).
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -379,18 +373,6 @@ inline void report(int fd, const char* who) {
     }
 }
 
-inline bool efence() {
-    static const bool on = [] { const char* e = getenv("NP_EFENCE"); return e && e[0] && e[0] != '0'; }();
-    return on;
-}
-
-struct FenceRec { void* base; size_t reserved, mapped; hipMemGenericAllocationHandle_t handle; };
-struct FenceTable {
-    std::mutex mu;
-    std::unordered_map<void*, FenceRec> live;
-};
-inline FenceTable& fence_table() { static FenceTable t; return t; }
-
 inline int poison() {      // -1: off
     static const int v = [] {
         const char* e = getenv("NP_DEVPOISON");
@@ -406,9 +388,8 @@ inline bool poison_runs() {      // NP_DEVPOISON=2: also the work buffers of a b
     return on;
 }
 
-inline hipError_t dev_malloc_raw(void** p, size_t bytes);
 inline hipError_t dev_malloc(void** p, size_t bytes) {
-    const hipError_t e = dev_malloc_raw(p, bytes);
+    const hipError_t e = dev_cache().get(p, bytes);
     if (e == hipSuccess) alloc_log("D+", *p, bytes);
     if (e == hipSuccess && poison() >= 0 && bytes) {
         (void)hipMemsetAsync(*p, poison(), bytes, nullptr);
@@ -417,64 +398,10 @@ inline hipError_t dev_malloc(void** p, size_t bytes) {
     return e;
 }
 
-inline hipError_t dev_malloc_raw(void** p, size_t bytes) {
-    if (!efence()) return dev_cache().get(p, bytes);
-    *p = nullptr;
-    int dev = 0;
-    hipError_t e = hipGetDevice(&dev);
-    if (e != hipSuccess) return e;
-    hipMemAllocationProp prop = {};
-    prop.type = hipMemAllocationTypePinned;
-    prop.location.type = hipMemLocationTypeDevice;
-    prop.location.id = dev;
-    size_t gran = 0;
-    e = hipMemGetAllocationGranularity(&gran, &prop, hipMemAllocationGranularityMinimum);
-    if (e != hipSuccess) return e;
-    if (gran == 0) gran = (size_t)2 << 20;
-    const size_t need = (bytes + 15) & ~(size_t)15;
-    const size_t mapped = ((need ? need : 16) + gran - 1) / gran * gran;
-    FenceRec r{nullptr, mapped + gran, mapped, {}};
-    e = hipMemAddressReserve(&r.base, r.reserved, gran, nullptr, 0);
-    if (e != hipSuccess) return e;
-    e = hipMemCreate(&r.handle, mapped, &prop, 0);
-    if (e != hipSuccess) { (void)hipMemAddressFree(r.base, r.reserved); return e; }
-    e = hipMemMap(r.base, mapped, 0, r.handle, 0);
-    if (e != hipSuccess) { (void)hipMemRelease(r.handle); (void)hipMemAddressFree(r.base, r.reserved); return e; }
-    hipMemAccessDesc acc = {};
-    acc.location = prop.location;
-    acc.flags = hipMemAccessFlagsProtReadWrite;
-    e = hipMemSetAccess(r.base, mapped, &acc, 1);
-    if (e != hipSuccess) { (void)hipMemUnmap(r.base, mapped); (void)hipMemRelease(r.handle); (void)hipMemAddressFree(r.base, r.reserved); return e; }
-    void* user = static_cast<char*>(r.base) + (mapped - need);
-    {
-        FenceTable& t = fence_table();
-        std::lock_guard<std::mutex> g(t.mu);
-        t.live[user] = r;
-    }
-    *p = user;
-    return hipSuccess;
-}
-
 inline hipError_t dev_free(void* p) {
     if (!p) return hipSuccess;
     alloc_log("D-", p, 0);
-    if (!efence()) return dev_cache().put(p);
-    FenceRec r;
-    {
-        FenceTable& t = fence_table();
-        std::lock_guard<std::mutex> g(t.mu);
-        auto it = t.live.find(p);
-        if (it == t.live.end()) return hipFree(p);      // (allocated before the mode was read: cannot happen, the flag is read once)
-        r = it->second;
-        t.live.erase(it);
-    }
-    (void)hipDeviceSynchronize();                        // hipFree waits for work in flight; so does this
-    (void)hipMemUnmap(r.base, r.mapped);
-    (void)hipMemRelease(r.handle);
-    // The address range is NOT handed back: a range that is reserved and mapped again showed stale contents on this runtime (ROCm 7.2:
-    // third reuse of one range: 43 % of a buffer wrong after a fill kernel + hipMemsetAsync), and a debugging
-    // mode can afford to leak address space (47 bits of it) -- a freed buffer's range also stays unmapped, so a use after free faults too.
-    return hipSuccess;
+    return dev_cache().put(p);
 }
 
 }  // namespace npalloc

@@ -63,3 +63,18 @@ def test_the_tools_hold_no_gpu_program_and_nothing_registers_memory_that_exists(
         if path.endswith((".hip", ".cpp", ".h", ".c")) and re.search(r"\bhipHostRegister\s*\(", text):
             bad.append(path)
     assert not bad, bad
+
+
+def test_device_memory_comes_from_plain_allocations():
+    # (no buffer is placed against an unmapped page: an access out of range is looked for in the host models, not by a fault)
+    bad = [path for path, text in texts() if path.startswith("nextpolish_amd") and re.search(r"\bhipMem(AddressReserve|Create|Map|SetAccess)\b", text)]
+    assert not bad, bad
+
+
+def test_every_switch_the_user_document_names_is_read():
+    src = "".join(text for path, text in texts() if path.startswith("nextpolish_amd") or path in ("bench.py",))
+    with open(os.path.join(ROOT, "INTEGRATION.md")) as f:
+        named = set(re.findall(r"\bNP[12]?_[A-Z][A-Z0-9_]*", f.read()))
+    assert len(named) > 20
+    bad = sorted(n for n in named if not re.search(r"(getenv|getenv_|env_\w+|environ\w*(?:\.get)?)[(\[]\s*\"%s\"" % n, src))
+    assert not bad, bad
