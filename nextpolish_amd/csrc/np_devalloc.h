@@ -10,8 +10,10 @@
 // library created (stream_create below keeps the registry) is asked with hipStreamQuery; for each one that is busy an event is
 // recorded and kept with the block, and the block is handed out again only once those events have completed (asked with
 // hipEventQuery at the time of the request; a block that is not ready is skipped, the request falls through to hipMalloc).
-// NP_DEVCACHE_MB=<n> bounds the idle bytes kept per device (default 16384; 0 = no cache: every release is a hipFree as before); over the
-// bound the largest idle blocks go back to the runtime, and when hipMalloc runs out of memory the cache is emptied and the request retried.
+// NP_DEVCACHE_MB=<n> bounds the idle bytes kept per device (default 16384, at least 256: with nothing kept, every release of the ~110 buffers
+// of a call would be one to the runtime, the pattern in which a process was seen to stop); NP_PINCACHE_MB=<n> the same for page-locked host
+// memory (default 2048).  Over the bound the largest idle blocks go back to the runtime, and when hipMalloc runs out of memory the cache is
+// emptied and the request retried.
 // Whenever memory does go back to the runtime, every stream is synchronised with hipStreamSynchronize first (quiesce below, and why).
 //
 // NP_DEVPOISON=1 (debugging; or a hex byte, e.g. NP_DEVPOISON=ff): every new device buffer is filled with that byte (default a5) before it
@@ -132,7 +134,7 @@ inline void busy_streams(int dev, std::vector<hipStream_t>* out) {
 
 // Before memory really goes back to the runtime.  hipFree and hipHostFree wait for work in flight on every stream, and a release was seen
 // not to return at all: three stops of the test process inside this project's own release path (DevBuf::ensure, np1_batch_free; the last
-// one in BlockCache::put, which with the cache off calls hipFree and nothing else), while hipStreamQuery answered "ready" for every stream
+// one in BlockCache::put with nothing kept, where it made one call, hipFree), while hipStreamQuery answered "ready" for every stream
 // of the process (profiles/r6_hang_hunt.txt).  hipStreamSynchronize was not seen to stop.  So every stream of the registry and the null
 // stream are synchronised with it first, under one lock so that two releasing threads do not interleave: the release itself then has no
 // work in flight to wait for.
@@ -169,42 +171,39 @@ public:
         int dev = 0;
         (void)hipGetDevice(&dev);
         const size_t want = size_class(bytes);
-        if (cap_) {
-            Block hit{};
-            bool found = false;
-            std::vector<hipEvent_t> done;
-            {
-                std::lock_guard<std::mutex> g(mu_);
-                auto& fl = free_list_[dev];
-                // a block of up to 1.5x the class (small ones: up to 4x, nothing is lost with them)
-                const size_t most = want < ((size_t)1 << 20) ? want * 4 : want + want / 2;
-                int looked = 0;
-                for (auto it = fl.lower_bound(want); it != fl.end() && it->first <= most && looked < 8; ++it, ++looked) {
-                    bool ready = true;
-                    for (hipEvent_t e : it->second.waits) if (hipEventQuery(e) != hipSuccess) { ready = false; break; }
-                    if (!ready) { ++st_.not_ready; continue; }
-                    hit = it->second;
-                    fl.erase(it);
-                    found = true;
-                    break;
-                }
-                if (found) {
-                    st_.cached -= hit.bytes;
-                    st_.live += hit.bytes;
-                    ++st_.hits;
-                    live_[hit.p] = Live{hit.bytes, dev};
-                    for (hipEvent_t e : hit.waits) spare_events_.push_back(e);
-                }
+        Block hit{};
+        bool found = false;
+        {
+            std::lock_guard<std::mutex> g(mu_);
+            auto& fl = free_list_[dev];
+            // a block of up to 1.5x the class (small ones: up to 4x, nothing is lost with them)
+            const size_t most = want < ((size_t)1 << 20) ? want * 4 : want + want / 2;
+            int looked = 0;
+            for (auto it = fl.lower_bound(want); it != fl.end() && it->first <= most && looked < 8; ++it, ++looked) {
+                bool ready = true;
+                for (hipEvent_t e : it->second.waits) if (hipEventQuery(e) != hipSuccess) { ready = false; break; }
+                if (!ready) { ++st_.not_ready; continue; }
+                hit = it->second;
+                fl.erase(it);
+                found = true;
+                break;
             }
-            if (found) { *p = hit.p; return hipSuccess; }
+            if (found) {
+                st_.cached -= hit.bytes;
+                st_.live += hit.bytes;
+                ++st_.hits;
+                live_[hit.p] = Live{hit.bytes, dev};
+                for (hipEvent_t e : hit.waits) spare_events_.push_back(e);
+            }
         }
-        hipError_t e = alloc_(p, cap_ ? want : bytes);
-        if (e != hipSuccess && cap_) {
+        if (found) { *p = hit.p; return hipSuccess; }
+        hipError_t e = alloc_(p, want);
+        if (e != hipSuccess) {
             (void)hipGetLastError();
             flush(dev);                      // out of memory with blocks of our own lying idle: give them back and ask again
             e = alloc_(p, want);
         }
-        if (e == hipSuccess && cap_) {
+        if (e == hipSuccess) {
             std::lock_guard<std::mutex> g(mu_);
             ++st_.misses;
             st_.live += want;
@@ -222,8 +221,8 @@ public:
             if (it == live_.end()) { ++st_.raw_frees; l.bytes = 0; }
             else { l = it->second; live_.erase(it); st_.live -= l.bytes; }
         }
-        if (!cap_ || l.bytes == 0 || l.bytes > cap_) {
-            if (cap_ && l.bytes) { std::lock_guard<std::mutex> g(mu_); ++st_.raw_frees; }
+        if (l.bytes == 0 || l.bytes > cap_) {
+            if (l.bytes) { std::lock_guard<std::mutex> g(mu_); ++st_.raw_frees; }
             std::lock_guard<std::mutex> g(raw_free_mutex());
             quiesce();
             return free_(p);
@@ -311,7 +310,8 @@ private:
 inline size_t env_mb(const char* name, size_t dflt_mb) {
     const char* e = getenv(name);
     if (!e || !e[0]) return dflt_mb << 20;
-    return (size_t)strtoull(e, nullptr, 10) << 20;
+    const size_t mb = (size_t)strtoull(e, nullptr, 10);
+    return mb < 256 ? (size_t)256 << 20 : mb > SIZE_MAX >> 20 ? SIZE_MAX : mb << 20;
 }
 inline hipError_t raw_dev_alloc(void** p, size_t n) { return hipMalloc(p, n); }
 inline hipError_t raw_dev_free(void* p) { return hipFree(p); }
