@@ -29,12 +29,14 @@
 #include <time.h>
 #include <unistd.h>
 
+#include <chrono>
 #include <cstdio>
 #include <cstdlib>
 #include <cstdint>
 #include <cstring>
 #include <map>
 #include <mutex>
+#include <shared_mutex>
 #include <unordered_map>
 #include <vector>
 
@@ -88,9 +90,11 @@ inline hipError_t host_free(void* p);
 
 // ----------------------------------------------------------------------------------------------- stream registry
 // Streams of both libraries are created and destroyed through here, so that a released block can be fenced against everything in flight
-// (BlockCache) and a stopped process can say which stream is busy (np_busy_streams, used by the tests' watchdog).
+// (BlockCache) and a stopped process can say which stream is busy (report below, used by the tests' watchdog).
+// Whoever asks, waits for or records on streams of the registry holds `mu` shared until it is done with them; stream_destroy takes it alone
+// to strike the stream off.  So a stream is never destroyed under a thread that releases memory at the same time.
 struct StreamRegistry {
-    std::mutex mu;
+    std::shared_timed_mutex mu;
     std::map<hipStream_t, int> live;      // stream -> device
 };
 inline StreamRegistry& stream_registry() { static StreamRegistry* r = new StreamRegistry(); return *r; }
@@ -100,7 +104,7 @@ inline hipError_t stream_create(hipStream_t* q) {
         int dev = 0;
         (void)hipGetDevice(&dev);
         StreamRegistry& R = stream_registry();
-        std::lock_guard<std::mutex> g(R.mu);
+        std::lock_guard<std::shared_timed_mutex> g(R.mu);
         R.live[*q] = dev;
     }
     return e;
@@ -114,22 +118,17 @@ inline hipError_t stream_destroy(hipStream_t q) {
     if (StreamDestroyHook h = stream_destroy_hook()) h(q);
     {
         StreamRegistry& R = stream_registry();
-        std::lock_guard<std::mutex> g(R.mu);
+        std::lock_guard<std::shared_timed_mutex> g(R.mu);
         R.live.erase(q);
     }
     return hipStreamDestroy(q);
 }
-// streams of `dev` (plus the null stream) that still have work in flight
-inline void busy_streams(int dev, std::vector<hipStream_t>* out) {
-    out->clear();
-    std::vector<hipStream_t> all;
-    {
-        StreamRegistry& R = stream_registry();
-        std::lock_guard<std::mutex> g(R.mu);
-        for (auto& kv : R.live) if (kv.second == dev) all.push_back(kv.first);
-    }
-    all.push_back(nullptr);
-    for (hipStream_t q : all) if (hipStreamQuery(q) == hipErrorNotReady) out->push_back(q);
+// f(q) for every stream of `dev` (and the null stream) that still has work in flight
+template <class F> inline void for_busy_streams(int dev, F f) {
+    StreamRegistry& R = stream_registry();
+    std::shared_lock<std::shared_timed_mutex> g(R.mu);
+    for (auto& kv : R.live) if (kv.second == dev && hipStreamQuery(kv.first) == hipErrorNotReady) f(kv.first);
+    if (hipStreamQuery(nullptr) == hipErrorNotReady) f((hipStream_t) nullptr);
 }
 
 // Before memory really goes back to the runtime.  hipFree and hipHostFree wait for work in flight on every stream, and a release was seen
@@ -140,13 +139,9 @@ inline void busy_streams(int dev, std::vector<hipStream_t>* out) {
 // work in flight to wait for.
 inline std::mutex& raw_free_mutex() { static std::mutex* m = new std::mutex(); return *m; }
 inline void quiesce() {
-    std::vector<hipStream_t> all;
-    {
-        StreamRegistry& R = stream_registry();
-        std::lock_guard<std::mutex> g(R.mu);
-        for (auto& kv : R.live) all.push_back(kv.first);
-    }
-    for (hipStream_t q : all) (void)hipStreamSynchronize(q);
+    StreamRegistry& R = stream_registry();
+    std::shared_lock<std::shared_timed_mutex> g(R.mu);
+    for (auto& kv : R.live) (void)hipStreamSynchronize(kv.first);
     (void)hipStreamSynchronize(nullptr);
 }
 
@@ -229,17 +224,15 @@ public:
         }
         // fence the block against whatever is in flight on any stream of ours (what hipFree did by waiting)
         Block b{p, l.bytes, {}};
-        std::vector<hipStream_t> busy;
-        busy_streams(l.dev, &busy);
-        for (hipStream_t q : busy) {
+        for_busy_streams(l.dev, [&](hipStream_t q) {
             hipEvent_t e = take_event();
             if (!e || hipEventRecord(e, q) != hipSuccess) {      // cannot fence: wait like hipFree would have
                 if (e) give_event(e);
                 (void)hipStreamSynchronize(q);
-                continue;
+                return;
             }
             b.waits.push_back(e);
-        }
+        });
         std::vector<Block> evict;
         {
             std::lock_guard<std::mutex> g(mu_);
@@ -350,18 +343,18 @@ inline hipError_t host_free(void* p) {
 // What a stopped process can say about itself (tests/conftest.py's watchdog calls np1_diag_report / np2_diag_report from a helper thread):
 // every stream of the registry with hipStreamQuery's answer, and the cache counters: whether the stopped thread still has work to wait for.
 inline void report(int fd, const char* who) {
-    std::vector<std::pair<hipStream_t, int>> all;
-    {
-        StreamRegistry& R = stream_registry();
-        std::lock_guard<std::mutex> g(R.mu);
-        for (auto& kv : R.live) all.emplace_back(kv.first, kv.second);
-    }
-    all.emplace_back(nullptr, -1);
-    dprintf(fd, "[np diag] %s: %zu stream(s) in the registry (+ the null stream)\n", who, all.size() - 1);
-    for (auto& kv : all) {
-        const hipError_t e = hipStreamQuery(kv.first);
-        dprintf(fd, "[np diag]   stream %p device %d: %s\n", (void*)kv.first, kv.second, e == hipSuccess ? "ready" : e == hipErrorNotReady ? "NOT READY" : hipGetErrorString(e));
-    }
+    StreamRegistry& R = stream_registry();
+    const auto line = [fd](hipStream_t q, int dev) {
+        const hipError_t e = hipStreamQuery(q);
+        dprintf(fd, "[np diag]   stream %p device %d: %s\n", (void*)q, dev, e == hipSuccess ? "ready" : e == hipErrorNotReady ? "NOT READY" : hipGetErrorString(e));
+    };
+    std::shared_lock<std::shared_timed_mutex> g(R.mu, std::chrono::seconds(2));
+    if (g.owns_lock()) {
+        dprintf(fd, "[np diag] %s: %zu stream(s) in the registry (+ the null stream)\n", who, R.live.size());
+        for (auto& kv : R.live) line(kv.first, kv.second);
+        g.unlock();
+    } else dprintf(fd, "[np diag] %s: a thread holds the stream registry\n", who);
+    line(nullptr, -1);
     (void)hipGetLastError();
     for (int k = 0; k < 2; ++k) {
         BlockCache& c = k ? host_cache() : dev_cache();

@@ -16,9 +16,30 @@ static int reuse() {
     return 0;
 }
 
+// A thread gives memory back (to the cache, or the cache's blocks to the runtime) while another destroys a stream.  Every runtime call takes
+// 40 ms, so the releasing thread is still at the first of five streams when the last of them is destroyed.
+static int beside_destroy(bool flush) {
+    hipStream_t q[5];
+    for (auto& s : q) if (npalloc::stream_create(&s) != hipSuccess) return 1;
+    void *kept = nullptr, *held = nullptr;
+    if (npalloc::dev_malloc(&kept, 4096) != hipSuccess || npalloc::dev_malloc(&held, 4096) != hipSuccess) return 1;
+    (void)npalloc::dev_free(kept);
+    hipStream_t last = npalloc::stream_registry().live.rbegin()->first;
+    for (auto& s : q) s->busy = true;
+    fake().slow_ms = 40;
+    std::thread releasing([&] { if (flush) npalloc::dev_cache().flush(-1); else (void)npalloc::dev_free(held); });
+    while (fake().in_call == 0) std::this_thread::yield();
+    (void)npalloc::stream_destroy(last);
+    releasing.join();
+    printf("used_destroyed %d left %d gone %d\n", fake().used_destroyed.load(), (int)npalloc::stream_registry().live.size(), last->gone ? 1 : 0);
+    return 0;
+}
+
 int main(int argc, char** argv) {
     const char* what = argc > 1 ? argv[1] : "";
     if (!strcmp(what, "reuse")) return reuse();
-    fprintf(stderr, "devalloc_host reuse\n");
+    if (!strcmp(what, "free_beside_destroy")) return beside_destroy(false);
+    if (!strcmp(what, "flush_beside_destroy")) return beside_destroy(true);
+    fprintf(stderr, "devalloc_host reuse|free_beside_destroy|flush_beside_destroy\n");
     return 2;
 }

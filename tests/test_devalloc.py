@@ -26,3 +26,9 @@ def test_buffers_taken_and_given_back_again_and_again_make_no_release(mb):
     got = run("reuse", **({} if mb is None else {"NP_DEVCACHE_MB": mb, "NP_PINCACHE_MB": mb}))
     assert got["frees"] == 0 and got["host_frees"] == 0, got
     assert 0 < got["mallocs"] <= 40 and 0 < got["host_mallocs"] <= 40, got
+
+
+@pytest.mark.parametrize("what", ["free_beside_destroy", "flush_beside_destroy"])
+def test_no_stream_is_used_by_a_release_after_another_thread_destroyed_it(what):
+    got = run(what)
+    assert got == {"used_destroyed": 0, "left": 4, "gone": 1}, got
