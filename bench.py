@@ -47,6 +47,16 @@ WORKLOADS = {
 }
 
 
+T_START = time.time()
+
+
+def step(what):
+    """One line on stderr when a part of the run has ended (stdout carries the JSON line alone)."""
+    if int(os.environ.get("RANK", "0")) == 0:
+        sys.stderr.write("[bench %6.1f s] %s\n" % (time.time() - T_START, what))
+        sys.stderr.flush()
+
+
 def contig_lengths(total, lo, hi, seed=20250117 + 3):
     rng = random.Random(seed)
     lens, acc = [], 0
@@ -167,6 +177,7 @@ def pmc_traffic(args, kernel_substr):
                                     "--steps", "1", "--warmup", "0", "--pmc-batches", str(args.pmc_batches)], ctr)
             hit = [v for k, v in rows.items() if kernel_substr in k]
             vals[ctr] = sum(a * n for a, n in hit) / max(1, sum(n for _a, n in hit))
+            step("counter pass %s" % ctr)
         except Exception as e:   # profiling is best effort: the bench line stays valid without it
             return None, "pmc pass failed: %r" % (e,)
     fetch_b, write_b = vals["FETCH_SIZE"] * 1024.0, vals["WRITE_SIZE"] * 1024.0
@@ -279,7 +290,7 @@ def lgs_leg(rank, local_rank, workers, contig_mb, calls, with_ref, with_pmc):
         f.write(bam + "\n")
     go = os.path.join(d, "go")
     env = dict(os.environ, NP2_DEVICE=str(local_rank))
-    wt = os.environ.get("NP2_WORKER_THREADS", "2")   # many workers share the host cores of one GPU (round-3 sweep: 24 x 2 > 16 x 4 > 12 x 4)
+    wt = os.environ.get("NP2_WORKER_THREADS", "2")   # many workers share the host cores of one GPU
     env["NP_HOST_THREADS"] = wt
     env["NP_IO_THREADS"] = wt
     lib2 = os.path.join(ROOT, "nextpolish_amd", "lib", "nextpolish2.so")
@@ -294,6 +305,7 @@ def lgs_leg(rank, local_rank, workers, contig_mb, calls, with_ref, with_pmc):
         time.sleep(0.01)
     open(go, "w").close()
     outs = [p.communicate() for p in ps]
+    step("long-read leg: %d workers x %d calls" % (workers, calls))
     bad = [o[1][-300:] for p, o in zip(ps, outs) if p.returncode != 0]
     if bad:
         shutil.rmtree(d, ignore_errors=True)
@@ -470,6 +482,7 @@ def _write_files(streams, fa, bam, qual_model):
     t0 = time.time()
     if L.np1_streams_write_files_q(arr, len(streams), fa.encode(), bam.encode(), 1, qual_model) != 0:
         raise RuntimeError(nat.last_error())
+    step("files written: %.0f MB of records" % (os.path.getsize(bam) / 1e6))
     return time.time() - t0
 
 
@@ -490,6 +503,7 @@ def _time_files(fa, bam, draft_bp, threads, n_records, cold_runs, warm_runs, pip
             raise RuntimeError("nextpolish1 scorechain failed")
         best = min(best, time.time() - t0)
         nbytes = n
+        step("from files, a new process")
     import ctypes as C
     from nextpolish_amd import _native as nat
     Ls = nat.lib()
@@ -518,6 +532,7 @@ def _time_files(fa, bam, draft_bp, threads, n_records, cold_runs, warm_runs, pip
             Ls.np1_pipe_ingest_stats(pipe.handle, stats, 1)      # (the first pass is not part of the decoder's figures either)
         nout = got[0]
     Ls.np1_pipe_ingest_stats(pipe.handle, stats, 1)
+    step("from files, %d passes of a running process" % (warm_runs + 1))
     size = os.path.getsize(bam)
     r = {"mbp_s": round(draft_bp / 1e6 / best, 2), "seconds": round(best, 3), "warm_mbp_s": round(draft_bp / 1e6 / warm, 2), "warm_seconds": round(warm, 3),
          "bam_mb": round(size / 1e6, 1), "bam_bytes_per_record": round(size / max(1, n_records), 2), "fasta_bytes_out": nbytes, "bases_out_warm": nout}
@@ -615,6 +630,7 @@ def parity_check(pipe, streams, budget_bp, per_batch_cap_bp=40000000, big_second
         got = C.string_at(p, ln.value)
         want = hashlib.md5(ob.score_chain(streams[k], c).encode()).hexdigest()
         oracle_md5[streams[k].names[c]] = want
+        step("contig of %d bp compared with the oracle" % L)
         return None if hashlib.md5(got).hexdigest() == want else streams[k].names[c]
     oracle_md5 = {}      # name -> md5 of the oracle's string: the from-files leg compares its own output of the same contigs with these
     with ThreadPoolExecutor(max(1, min(host_cores(), len(chosen)))) as ex:
@@ -643,7 +659,7 @@ def main():
     ap.add_argument("--pmc-batches", type=int, default=4, help="batches of the workload the two rocprofv3 --pmc child runs polish (generating all 600 M records twice more is most of a full-size run)")
     ap.add_argument("--no-e2e", action="store_true", help="skip the from-files leg")
     ap.add_argument("--no-lgs", action="store_true", help="skip the long-read (nextpolish2) leg")
-    ap.add_argument("--lgs-workers", type=int, default=24, help="worker processes per GPU of the long-read leg (x NP2_WORKER_THREADS host threads each, default 2)")
+    ap.add_argument("--lgs-workers", type=int, default=14, help="worker processes per GPU of the long-read leg (x NP2_WORKER_THREADS host threads each, default 2); with this process and its helpers at most 16 processes share a card")
     ap.add_argument("--lgs-mb", type=float, default=5.0, help="contig length (Mb) each long-read worker polishes")
     ap.add_argument("--lgs-calls", type=int, default=24, help="timed calls per long-read worker (the rate is bp over the span from the common start to the last end; measured: 0.63 s of ramp and stragglers + 0.70 s per round of calls, so 4 / 8 calls read 140 / 154 Mbp/s of a steady state of 171: a worker of a real run polishes hundreds of windows)")
     ap.add_argument("--no-lgs-config4", action="store_true", help="skip the 100 Mb / 67-contig long-read run (BASELINE configs[3] at its stated size)")
@@ -692,8 +708,11 @@ def main():
     # chromosome-sized contigs are generated segment by segment on all of the rank's threads (np_synth.cpp): few streams at a time
     outer = 2 if max(lens) >= (16 << 20) else max(1, min(per_rank, len(blens)))
     with ThreadPoolExecutor(outer) as ex:
-        streams = list(ex.map(lambda k: nat.Stream.synth(blens[k], depth=depth, seed=20250117 + 1000 * int(batches[k][0][1:]),
-                                                         prefix="b%dc" % int(batches[k][0][1:])), range(len(blens))))
+        streams = []
+        for s in ex.map(lambda k: nat.Stream.synth(blens[k], depth=depth, seed=20250117 + 1000 * int(batches[k][0][1:]),
+                                                   prefix="b%dc" % int(batches[k][0][1:])), range(len(blens))):
+            streams.append(s)
+            step("records of batch %d of %d generated" % (len(streams), len(blens)))
     t_gen = time.time() - t_gen
     n_reads = sum(s.n_reads for s in streams)
     alg_in = [s.algorithmic_bytes(False) for s in streams]   # records (32 + 4 n_cigar + ceil(l/2)) + draft, per batch
@@ -711,6 +730,7 @@ def main():
     for s in streams:
         s.pin()
     t_pin = time.time() - t_pin
+    step("upload forms built, streams page-locked")
     pipe = Pipe(local_rank, lanes=args.lanes)
     cfg = nat.default_config()
     L = nat.lib()
@@ -753,6 +773,7 @@ def main():
         pipe.run(streams, cfg=cfg, fetch=False)
     sync_all()
     dt_str = max_over_ranks(time.perf_counter() - t0)
+    step("%d streamed passes" % args.streamed_passes)
     L.np1_stream_upload_bytes.restype = C.c_uint64
     L.np1_stream_upload_bytes.argtypes = [C.c_void_p]
     h2d_bytes = sum(int(L.np1_stream_upload_bytes(s.handle)) for s in streams)   # what really crosses PCIe per pass (2-bit bases, 16-bit counts, no offsets)
@@ -769,6 +790,7 @@ def main():
     resident(args.steps)
     sync_all()
     dt = max_over_ranks(time.perf_counter() - t0)
+    step("%d warm-up and %d timed steps" % (args.warmup, args.steps))
 
     # ---- per-stage HIP-event timing on the pipeline's own stream (separate instrumented passes, one lane, batch by batch)
     stage_acc, launches, polished, updates = {}, 0, [], 0
@@ -804,6 +826,7 @@ def main():
         pipe.close()
         pipe = None
         e2e = e2e_from_files(streams, draft_bp_total, ncpu, n_reads, expect=(parity or {}).get("oracle_md5"))
+        step("from-files leg")
     if pipe is not None:
         pipe.close()
     lgs = None
@@ -829,6 +852,7 @@ def main():
             # consensus, every contig compared with the md5 the compiled reference produced (tests/tools/check_config4.py, tests/golden/)
             env4 = dict(os.environ, NP2_DEVICE=str(local_rank), NP_HOST_THREADS=os.environ.get("NP2_WORKER_THREADS", "2"), NP_IO_THREADS=os.environ.get("NP2_WORKER_THREADS", "2"))
             q = subprocess.run([sys.executable, os.path.join(ROOT, "tests", "tools", "check_config4.py"), "--procs", "8"], capture_output=True, text=True, env=env4)
+            step("long-read draft of 67 contigs")
             try:
                 c4 = json.loads(q.stdout.strip().splitlines()[-1])
                 lgs["config4"] = {"mbp_s": c4.get("mbp_s"), "draft_bp": c4.get("draft_bp"), "contigs": c4.get("contigs"), "groups": c4.get("groups"), "procs": c4.get("procs"),
@@ -901,6 +925,7 @@ def main():
                         out["lgs"][k] = lgs[k]
         if world == 1 and not args.no_cpu_baseline:
             out["cpu_baseline"] = cpu_baseline(depth, args.cpu_sample_mb, ncpu)
+            step("CPU baseline")
         if world == 1 and not args.no_phase:
             try:
                 out["snp_phase"] = phase_leg(local_rank, args.phase_mb, 3, ncpu, not args.no_cpu_baseline)
