@@ -89,7 +89,7 @@ struct LdsTab {
     __device__ __forceinline__ uint16_t rd(uint32_t i) const { return col[i << 6]; }
     __device__ __forceinline__ void wr(uint32_t i, uint16_t v) { col[i << 6] = v; }
 };
-template <int LB, int DB, int DBG = 0>
+template <int LB, int DB>
 __global__ __launch_bounds__(64) void k_inflate_lds(const uint8_t* __restrict__ comp, const npdev::BlockDesc* __restrict__ blocks, uint32_t n_blocks, uint8_t* out,
                                                     uint32_t* __restrict__ status, nplds::Scratch* __restrict__ scratch) {
     __shared__ uint16_t slots[64u * nplds::Layout<LB, DB>::SLOTS];
@@ -99,7 +99,7 @@ __global__ __launch_bounds__(64) void k_inflate_lds(const uint8_t* __restrict__ 
     for (uint32_t b = me; b < n_blocks; b += lanes) {
         const npdev::BlockDesc d = blocks[b];
         int rc = 0;
-        if (d.out_len) rc = nplds::inflate_block<LB, DB, LdsTab, DBG>(comp + d.in_off, d.in_len, out + d.out_off, d.out_len, tab, sc);
+        if (d.out_len) rc = nplds::inflate_block<LB, DB, LdsTab>(comp + d.in_off, d.in_len, out + d.out_off, d.out_len, tab, sc);
         status[b] = (uint32_t)rc;
     }
 }
@@ -118,13 +118,6 @@ int launch_inflate_lds(hipStream_t q, const uint8_t* comp, const npdev::BlockDes
     const uint32_t per_cu = std::max<uint32_t>(1u, std::min<uint32_t>(cap_per_cu, 163840u / lds_bytes));
     const uint32_t waves = std::min<uint32_t>(cus * per_cu, (n_blocks + 63u) / 64u);
     if (scratch.ensure((size_t)waves * 64u * sizeof(nplds::Scratch))) return -1;
-    // NP1_LDS_DBG=<bits>: timing experiments with parts of the work left out (np_inflate_lds.h; the output is wrong)
-    static const int dbg = getenv("NP1_LDS_DBG") ? atoi(getenv("NP1_LDS_DBG")) : 0;
-    if constexpr (LB == 7 && DB == 5) {      // (the experiment builds exist for the default table sizes only)
-        if (dbg == 1) { k_inflate_lds<LB, DB, 1><<<waves, 64, 0, q>>>(comp, blocks, n_blocks, out, status, scratch.as<nplds::Scratch>()); return 0; }
-        if (dbg == 2) { k_inflate_lds<LB, DB, 2><<<waves, 64, 0, q>>>(comp, blocks, n_blocks, out, status, scratch.as<nplds::Scratch>()); return 0; }
-        if (dbg == 3) { k_inflate_lds<LB, DB, 3><<<waves, 64, 0, q>>>(comp, blocks, n_blocks, out, status, scratch.as<nplds::Scratch>()); return 0; }
-    }
     k_inflate_lds<LB, DB><<<waves, 64, 0, q>>>(comp, blocks, n_blocks, out, status, scratch.as<nplds::Scratch>());
     return 0;
 }

@@ -423,13 +423,13 @@ __device__ __forceinline__ void tile_epilogue(const VoteLane<E>& vl, const uint3
 template <int E>
 __device__ __forceinline__ void vote_part(const uint32_t* d, const SeqLds& sq, bool valid, uint32_t s, uint32_t g,
                                           int32_t jj, int lane, uint32_t& rsym, uint32_t& basemask, VoteLane<E>& vl,
-                                          uint32_t* L, uint32_t ablate = 0) {
+                                          uint32_t* L) {
     const bool cov = valid && s >= d[0] && s <= d[1];
-    if (cov) rsym = (ablate & 8u) ? (g & 0xfu) : desc_symbol(d, g, jj, sq);
+    if (cov) rsym = desc_symbol(d, g, jj, sq);
     const uint32_t p1 = wave_shr1(rsym), p2 = wave_shr1(p1);
     if (cov) {
         basemask |= 1u << rsym;
-        if (lane >= 2 && !(ablate & 4u)) vl.tally(p2 << 8 | p1 << 4 | rsym, L, lane);
+        if (lane >= 2) vl.tally(p2 << 8 | p1 << 4 | rsym, L, lane);
     }
 }
 
@@ -448,7 +448,7 @@ __global__ __launch_bounds__(NW * 64) void k_tile3(ReadsDev R, const uint32_t* _
                                                    uint32_t* __restrict__ heads, uint32_t heads_cap,
                                                    uint32_t* __restrict__ redo_out,
                                                    uint32_t redo_ci, uint32_t flag_single,
-                                                   unsigned long long* __restrict__ votes, uint32_t ablate) {
+                                                   unsigned long long* __restrict__ votes) {
     extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
     __shared__ __attribute__((aligned(16))) uint32_t sh_r[4];
     uint32_t* lists = lds;                             // NW * (E-2) * 64
@@ -521,7 +521,7 @@ __global__ __launch_bounds__(NW * 64) void k_tile3(ReadsDev R, const uint32_t* _
             const uint32_t sq0_lo = (uint32_t)sq0;   // descriptors carry the low word of their record's pool offset
             __syncthreads();
             // ---- this wave's chunk votes over the batch, in record order
-            if (chunk_ok && !(ablate & 2u)) {
+            if (chunk_ok) {
                 uint32_t a = nb, b = 0;
                 for (uint32_t base = 0; base < nb; base += 64) {
                     const uint32_t i = base + lane;
@@ -537,7 +537,7 @@ __global__ __launch_bounds__(NW * 64) void k_tile3(ReadsDev R, const uint32_t* _
                         if (hi > b) b = hi;
                     }
                 }
-                if (a < nb && !(ablate & 16u)) {
+                if (a < nb) {
                     const uint8_t* seqb = reinterpret_cast<const uint8_t*>(seqst);
                     // descriptor head (sfirst, slast, counts, base offset) and first segment of record a; the loop
                     // fetches record i+1's while it votes record i (one spare descriptor slot keeps the loads in range)
@@ -546,7 +546,7 @@ __global__ __launch_bounds__(NW * 64) void k_tile3(ReadsDev R, const uint32_t* _
                     for (uint32_t i = a; i <= b; ++i) {
                         const uint4 hn = *reinterpret_cast<const uint4*>(dsc + (i + 1) * DESC_WORDS);
                         const uint2 sgn = *reinterpret_cast<const uint2*>(dsc + (i + 1) * DESC_WORDS + DESC_SEG0);
-                        if (!(h.z & DESC_CHAIN) && !(ablate & 32u)) {
+                        if (!(h.z & DESC_CHAIN)) {
                             // wave-uniform shape test; the body is branch-free apart from uniform trip counts
                             const uint32_t nseg = h.z & 0xffu, nins = (h.z >> 8) & 0xffu;
                             const bool cov = sv >= h.x && sv <= h.y;
@@ -1386,10 +1386,6 @@ void launch_desc(hipStream_t st, const ReadsDev& R, int64_t n_reads, const uint3
     k_desc<<<nblk(n_reads, 256), 256, 0, st>>>(R, n_reads, ctg_off, soff, qs, qe, desc, ovf_pool, ovf_cap, chunk_first,
                                                chunk_last, counters);
 }
-static uint32_t ablate_env() {   // timing experiments only (results are wrong when set)
-    static const uint32_t v = getenv("NP1_ABLATE") ? (uint32_t)atoi(getenv("NP1_ABLATE")) : 0u;
-    return v;
-}
 
 int launch_tile3(hipStream_t st, int level, const ReadsDev& R, const uint32_t* soff, const uint32_t* desc,
                  const uint32_t* ovf_pool, const uint32_t* chunk_first, const uint32_t* chunk_last, uint32_t n_chunks, const uint32_t* redo_in,
@@ -1399,7 +1395,6 @@ int launch_tile3(hipStream_t st, int level, const ReadsDev& R, const uint32_t* s
                  unsigned long long* votes) {
     const uint32_t seq_w = (((max_lq + 1) >> 1) + 3) / 4 + 1;   // packed bases per record, in words (upper bound)
     const uint32_t per = (uint32_t)DESC_WORDS + seq_w;
-    const uint32_t ablate = ablate_env();
 #define NP1_TILE3(EE, NWW, BUDGET)                                                                                   \
     do {                                                                                                             \
         const uint32_t fixed = (uint32_t)(NWW) * (uint32_t)((EE)-2) * 64u + 8u + (uint32_t)DESC_WORDS;               \
@@ -1421,7 +1416,7 @@ int launch_tile3(hipStream_t st, int level, const ReadsDev& R, const uint32_t* s
                                                           redo_in,                                                   \
                                                           items, slot_info, slot_g, S, seq_w, nb_max, slot_res,      \
                                                           slot_rec, pool, pool_cap, counters, heads, heads_cap,      \
-                                                          redo_out, redo_ci, flag_single, votes, ablate);            \
+                                                          redo_out, redo_ci, flag_single, votes);                    \
     } while (0)
     if (level == 0) NP1_TILE3(8, 8, 13312u);        // 52 KiB: three workgroups per CU
     else if (level == 1) NP1_TILE3(64, 1, 13312u);

@@ -267,8 +267,7 @@ NPD_HD void load32(const uint8_t* p, const uint8_t* limit, uint32_t n, uint64_t*
 }
 
 // src[0 .. src_len): raw DEFLATE stream; dst[0 .. dst_len): its output; tab: Layout<LB, DB>::SLOTS 16-bit slots; sc: the lane's scratch.
-// (DBG: timing experiments only -- bit 0 drops the literal stores, bit 1 the match copies: wrong output)
-template <int LB, int DB, class Tab, int DBG = 0>
+template <int LB, int DB, class Tab>
 NPD_HD int inflate_block(const uint8_t* src, uint32_t src_len, uint8_t* dst, uint32_t dst_len, Tab& tab, Scratch* sc) {
     typedef Layout<LB, DB> Y;
     constexpr int CLB = 7 <= LB ? 7 : LB;      // primary bits of the code-length alphabet (its codes have up to 7 bits)
@@ -289,10 +288,8 @@ NPD_HD int inflate_block(const uint8_t* src, uint32_t src_len, uint8_t* dst, uin
     // own future output, written again later)
     auto flush = [&]() {
         if (!npend) return;
-        if (!(DBG & 1)) {
-            if ((size_t)(out_end - out) >= 8) *reinterpret_cast<u64u*>(out) = pend;
-            else for (uint32_t i = 0; i < npend; ++i) out[i] = (uint8_t)(pend >> (8 * i));
-        }
+        if ((size_t)(out_end - out) >= 8) *reinterpret_cast<u64u*>(out) = pend;
+        else for (uint32_t i = 0; i < npend; ++i) out[i] = (uint8_t)(pend >> (8 * i));
         out += npend;
         pend = 0;
         npend = 0;
@@ -374,7 +371,7 @@ NPD_HD int inflate_block(const uint8_t* src, uint32_t src_len, uint8_t* dst, uin
             if (c_rem) {
                 uint32_t piece = c_rem < 32 ? c_rem : 32;
                 if (c_off < piece) piece = c_off;
-                if (!(DBG & 2)) load32(c_dst - c_off, out_end, piece, &a0, &a1, &a2, &a3);
+                load32(c_dst - c_off, out_end, piece, &a0, &a1, &a2, &a3);
                 f_n = piece;
                 f_d = c_dst;
                 c_dst += piece;
@@ -393,7 +390,7 @@ NPD_HD int inflate_block(const uint8_t* src, uint32_t src_len, uint8_t* dst, uin
                     pend |= (uint64_t)sym << (8 * npend);
                     last8 = last8 >> 8 | (uint64_t)sym << 56;
                     nvalid = nvalid < 8 ? nvalid + 1 : 8;
-                    if (++npend == 8) { if (!(DBG & 1)) *reinterpret_cast<u64u*>(out) = pend; out += 8; pend = 0; npend = 0; }
+                    if (++npend == 8) { *reinterpret_cast<u64u*>(out) = pend; out += 8; pend = 0; npend = 0; }
                 } else if (sym == 256) {
                     ended = true;
                 } else {
@@ -411,14 +408,12 @@ NPD_HD int inflate_block(const uint8_t* src, uint32_t src_len, uint8_t* dst, uin
                         // a run: the period is the top `off` bytes of last8; whole words, each starting at the head of a period (what a word
                         // writes beyond the run is this lane's own future output), the end of the block byte by byte
                         const uint64_t x = off == 1 ? (last8 >> 56) * 0x0101010101010101ull : periodic(last8 >> (8 * (8 - off)), off, 0);
-                        if (!(DBG & 2)) {
-                            const uint32_t step = off == 3 || off == 6 ? 6u : off == 5 ? 5u : off == 7 ? 7u : 8u;
-                            uint32_t done = 0;
-                            for (; done < len && (size_t)(out_end - (out + done)) >= 8; done += step) *reinterpret_cast<u64u*>(out + done) = x;
-                            if (done < len) {
-                                uint32_t k = done % off;
-                                for (uint32_t i = done; i < len; ++i) { out[i] = (uint8_t)(x >> (8 * k)); if (++k == off) k = 0; }
-                            }
+                        const uint32_t step = off == 3 || off == 6 ? 6u : off == 5 ? 5u : off == 7 ? 7u : 8u;
+                        uint32_t done = 0;
+                        for (; done < len && (size_t)(out_end - (out + done)) >= 8; done += step) *reinterpret_cast<u64u*>(out + done) = x;
+                        if (done < len) {
+                            uint32_t k = done % off;
+                            for (uint32_t i = done; i < len; ++i) { out[i] = (uint8_t)(x >> (8 * k)); if (++k == off) k = 0; }
                         }
                         if (len >= 8) { last8 = off == 1 ? x : periodic(x, off, (len - 8) % off); nvalid = 8; }
                         else { last8 = last8 >> (8 * len) | x << (8 * (8 - len)); nvalid = nvalid + len < 8 ? nvalid + len : 8; }
@@ -436,21 +431,19 @@ NPD_HD int inflate_block(const uint8_t* src, uint32_t src_len, uint8_t* dst, uin
             // stored, exactly its bytes, and the window's next words are asked for
             b.slide_take();
             if (f_n) {
-                if (!(DBG & 2)) {
-                    // exactly f_n <= 32 bytes in as few stores as their count has bits (16 + 8 + 4 + 2 + 1): every store instruction is a transaction
-                    // per lane, and the decoder runs at about half of L2's transaction rate (profiles/r6_inflate_lds.txt item 10); byte by byte the
-                    // last n < 8 bytes alone were up to seven
-                    uint8_t* d = f_d;
-                    const uint32_t n = f_n;
-                    uint64_t w0 = a0, w1 = a1, w2 = a2, w3 = a3;
-                    if (n >= 16u) { store16(d, w0, w1); d += 16; w0 = w2; w1 = w3; }
-                    if (n == 32u) { store16(d, w0, w1); }
-                    else {
-                        if (n & 8u) { *reinterpret_cast<u64u*>(d) = w0; d += 8; w0 = w1; }
-                        if (n & 4u) { *reinterpret_cast<u32u*>(d) = (uint32_t)w0; d += 4; w0 >>= 32; }
-                        if (n & 2u) { *reinterpret_cast<u16u*>(d) = (uint16_t)w0; d += 2; w0 >>= 16; }
-                        if (n & 1u) *d = (uint8_t)w0;
-                    }
+                // exactly f_n <= 32 bytes in as few stores as their count has bits (16 + 8 + 4 + 2 + 1): every store instruction is a transaction
+                // per lane, and the decoder runs at about half of L2's transaction rate (profiles/r6_inflate_lds.txt item 10); byte by byte the
+                // last n < 8 bytes alone were up to seven
+                uint8_t* d = f_d;
+                const uint32_t n = f_n;
+                uint64_t w0 = a0, w1 = a1, w2 = a2, w3 = a3;
+                if (n >= 16u) { store16(d, w0, w1); d += 16; w0 = w2; w1 = w3; }
+                if (n == 32u) { store16(d, w0, w1); }
+                else {
+                    if (n & 8u) { *reinterpret_cast<u64u*>(d) = w0; d += 8; w0 = w1; }
+                    if (n & 4u) { *reinterpret_cast<u32u*>(d) = (uint32_t)w0; d += 4; w0 >>= 32; }
+                    if (n & 2u) { *reinterpret_cast<u16u*>(d) = (uint16_t)w0; d += 2; w0 >>= 16; }
+                    if (n & 1u) *d = (uint8_t)w0;
                 }
                 f_n = 0;
             }

@@ -78,3 +78,11 @@ def test_every_switch_the_user_document_names_is_read():
     assert len(named) > 20
     bad = sorted(n for n in named if not re.search(r"(getenv|getenv_|env_\w+|environ\w*(?:\.get)?)[(\[]\s*\"%s\"" % n, src))
     assert not bad, bad
+
+
+def test_no_switch_makes_a_result_wrong():
+    # a build that leaves work out to time the rest is no part of the tree
+    said = re.compile(r"results are wrong when|output is wrong|wrong output|experiments with wrong results|parts of the work left out")
+    bad = ["%s:%d" % (path, k) for path, text in texts() if path.startswith(("nextpolish_amd", "include", "bench.py"))
+           for k, line in enumerate(text.splitlines(), 1) if said.search(line)]
+    assert not bad, bad
