@@ -191,10 +191,6 @@ template <class C> struct Table {
     int32_t* TS;
     uint32_t* TF;
     uint32_t cap;
-    uint32_t* dbg;      // debugging (NP2_POA_DEBUG): where this wave is -- {stage, counter} -- readable from the host while the kernel runs
-    __device__ __forceinline__ void mark(uint32_t stage, uint32_t v) const {
-        if (dbg && __lane_id() == 0) { __atomic_store_n(dbg, stage, __ATOMIC_RELAXED); __atomic_store_n(dbg + 1, v, __ATOMIC_RELAXED); }
-    }
     __device__ __forceinline__ uint32_t capacity() const { if constexpr (C::TAB_LDS > 0) return C::TAB_LDS; else return cap; }
     __device__ __forceinline__ int32_t score(uint32_t i) const { if constexpr (C::TAB_LDS > 0) return (int32_t)L->ts[i]; else return TS[i]; }
     __device__ __forceinline__ uint32_t from(uint32_t i) const { if constexpr (C::TAB_LDS > 0) return (uint32_t)L->tf[i]; else return TF[i]; }
@@ -224,7 +220,6 @@ template <class C> __device__ void add_string(Graph<C>& G, uint32_t q, const cha
     if constexpr (BIGC) lds_sync(); else T.sync();
     // rows in emission order
     for (uint32_t r = 0; r < n; ++r) {
-        T.mark(3, q << 16 | r);
         const uint32_t v = uni(L->order[r]);
         const char vb = (char)uni(L->base[v]);
         const uint32_t row = r + 1;
@@ -328,7 +323,6 @@ template <class C> __device__ void add_string(Graph<C>& G, uint32_t q, const cha
     uint32_t np = 0;
     int32_t lowest_chr = -1, highest_chr = -1;
     for (uint32_t col = len; row != 0 || col != 0;) {
-        T.mark(4, row << 16 | col);
         const uint32_t from = uni(T.from(row * width + col));
         const uint32_t from_row = from >> FS, from_col = from & FMASK;
         int32_t node = -1, chr = -1;
@@ -353,7 +347,6 @@ template <class C> __device__ void add_string(Graph<C>& G, uint32_t q, const cha
     if (highest_chr < (int32_t)len - 1)                                                         // and behind the last one (the run takes the
         G.chain(q, s + highest_chr + 1, (uint32_t)((int32_t)len - highest_chr), &tail_first, &cur);   // terminator along, like the reference)
     for (uint32_t k = np; k-- > 0 && !G.fail;) {
-        T.mark(5, q << 16 | k);
         const int32_t chr = unis((int32_t)L->path_chr[k]);
         if (chr == -1) continue;
         const int32_t node = unis((int32_t)L->path_node[k]);
@@ -382,14 +375,12 @@ template <class C> __device__ void add_string(Graph<C>& G, uint32_t q, const cha
         if (first == -1) first = prev;
     }
     if (tail_first != -1 && !G.fail) G.connect((uint32_t)prev, (uint32_t)tail_first, q);
-    T.mark(6, q << 16 | G.n);
     if (!G.fail) G.reorder();
-    T.mark(7, q);
 }
 
 // the whole job: strings of one region -> consensus characters; returns false when the region has to go to the host version
 template <class C> __device__ bool poa_region(const char* pool, const uint32_t* __restrict__ str_off, const uint32_t* __restrict__ str_len, const Job& J, int32_t* TS, uint32_t* TF,
-                                              uint32_t tab_cap, char* out_pool, uint32_t* out_len, PoaLdsT<C>* L, uint32_t* dbg = nullptr) {
+                                              uint32_t tab_cap, char* out_pool, uint32_t* out_len, PoaLdsT<C>* L) {
     constexpr uint32_t NONE16 = C::NONE, MAXLEN = C::MAXLEN, MAXN = C::MAXN;
     using ix_t = typename C::ix;
     using path_t = typename C::path_t;
@@ -398,8 +389,7 @@ template <class C> __device__ bool poa_region(const char* pool, const uint32_t* 
     const uint32_t lane = __lane_id();
     if (J.n_str > C::MAXSTR) return false;
     Graph<C> G{L, 0u, 0u, 0u, false};
-    const Table<C> T{L, TS, TF, tab_cap, dbg};
-    T.mark(1, J.first_str);
+    const Table<C> T{L, TS, TF, tab_cap};
     // the first string is the graph: a chain, every node a group of its own, emission order = string order
     const uint32_t len0 = str_len[J.first_str];
     const char* s0 = pool + str_off[J.first_str];
@@ -426,7 +416,6 @@ template <class C> __device__ bool poa_region(const char* pool, const uint32_t* 
     int32_t top = -1;
     double carried = -1, top_score = -1;
     for (uint32_t r = 0; r < G.n; ++r) {
-        T.mark(8, r);
         const uint32_t v = uni(L->order[r]);
         int32_t from = -1;
         const uint32_t e0 = uni(L->in_head[v]);
@@ -451,9 +440,7 @@ template <class C> __device__ bool poa_region(const char* pool, const uint32_t* 
     // characters from the end of the path backwards, then turned over; an embedded terminator (a tail node built from the NUL of
     // a candidate) ends the string
     uint32_t m = 0;
-    T.mark(9, (uint32_t)top);
     for (int32_t v = top; v != -1; v = unis((int32_t)L->came_from[v])) ++m;
-    T.mark(10, m);
     if (m > J.out_cap) return false;
     char* out = out_pool + J.out_off;
     uint32_t k = m;
@@ -468,7 +455,6 @@ template <class C> __device__ bool poa_region(const char* pool, const uint32_t* 
         if (nul) { z = cb + (uint32_t)__ffsll((long long)nul) - 1u; break; }
     }
     if (lane == 0) *out_len = z;
-    T.mark(11, z);
     return true;
 }
 

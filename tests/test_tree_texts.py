@@ -86,3 +86,13 @@ def test_no_switch_makes_a_result_wrong():
     bad = ["%s:%d" % (path, k) for path, text in texts() if path.startswith(("nextpolish_amd", "include", "bench.py"))
            for k, line in enumerate(text.splitlines(), 1) if said.search(line)]
     assert not bad, bad
+
+
+def test_no_device_source_ends_the_process():
+    # (the drop-in symbols exit where the reference's do, on the host; code that launches kernels could leave them running behind it)
+    bad = []
+    for path, text in texts():
+        if path.startswith("nextpolish_amd/csrc") and path.endswith(".hip"):
+            if re.search(r"\b(_exit|_Exit|quick_exit|exit|abort)\s*\(", re.sub(r"//[^\n]*", "", text)):
+                bad.append(path)
+    assert not bad, bad

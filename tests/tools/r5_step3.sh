@@ -14,7 +14,7 @@ G = rb.bind("$R/nextpolish_amd/lib/nextpolish2.so")
 for _ in range(2):
     rb.polish(G, "/tmp/np2case/g.fa", "/tmp/np2case/bam.fofn", read_type=1)
 PY
-NP2_POA_DEBUG=1 NP2_POA_CHECK=1 NP2_TIMING=1 NP_HOST_THREADS=8 NP_IO_THREADS=8 timeout 150 python /tmp/np2case/run.py 2>&1 | grep -a "np2 poa" | tail -4
+NP2_POA_CHECK=1 NP2_TIMING=1 NP_HOST_THREADS=8 NP_IO_THREADS=8 timeout 150 python /tmp/np2case/run.py 2>&1 | grep -a "np2 poa" | tail -4
 ( export NP_HOST_THREADS=8 NP_IO_THREADS=8; cd /tmp && export TMPDIR=/tmp && timeout 200 rocprofv3 --kernel-trace --stats -d $O/ks -o ks -- python /tmp/np2case/run.py > /dev/null 2>&1 )
 python tools/rocprof_summary.py stats $O/ks/ks_results.db > $O/np2_kernel_stats_5mb.txt 2>&1; rm -rf $O/ks
 head -16 $O/np2_kernel_stats_5mb.txt | cut -c1-120
