@@ -7,5 +7,4 @@ mkdir -p $O
 timeout 500 python -m pytest tests/test_gpu_tiling.py "tests/test_gpu_score_chain.py::test_dropin_abi_and_cli" -x -q -m gpu -p no:cacheprovider > $O/tiling_tests.log 2>&1; echo "tiling + dropin rc=$? $(tail -1 $O/tiling_tests.log)"; grep -a -E "Error|assert|FAILED" $O/tiling_tests.log | head -8
 timeout 200 python __graft_entry__.py smoke > $O/smoke.log 2>&1; echo "smoke rc=$?"; tail -5 $O/smoke.log | cut -c1-200
 timeout 300 python -m pytest tests/test_gpu_np2.py -x -q -m gpu -p no:cacheprovider > $O/np2_tests.log 2>&1; echo "np2 tests rc=$? $(tail -1 $O/np2_tests.log)"
-timeout 200 python tests/tools/r4_lgs_quick.py 24 12 2> $O/lgs_quick.err | cut -c1-400
-NP2_PAGEABLE_RECORDS=1 timeout 200 python tests/tools/r4_lgs_quick.py 24 12 2>> $O/lgs_quick.err | cut -c1-400
+timeout 200 python tests/tools/r4_lgs_quick.py 14 12 2> $O/lgs_quick.err | cut -c1-400
