@@ -71,13 +71,15 @@ def test_device_memory_comes_from_plain_allocations():
     assert not bad, bad
 
 
-def test_every_switch_the_user_document_names_is_read():
+def test_the_user_document_names_the_switches_that_are_read_and_no_others():
     src = "".join(text for path, text in texts() if path.startswith("nextpolish_amd") or path in ("bench.py",))
+    read = re.compile(r'(?:getenv|env_\w+|environ\w*(?:\.get)?)[(\[]\s*"(NP[12]?_[A-Z][A-Z0-9_]*)"')
     with open(os.path.join(ROOT, "INTEGRATION.md")) as f:
         named = set(re.findall(r"\bNP[12]?_[A-Z][A-Z0-9_]*", f.read()))
-    assert len(named) > 20
-    bad = sorted(n for n in named if not re.search(r"(getenv|getenv_|env_\w+|environ\w*(?:\.get)?)[(\[]\s*\"%s\"" % n, src))
-    assert not bad, bad
+    libs = set(read.findall("".join(text for path, text in texts() if path.startswith("nextpolish_amd"))))
+    assert len(named) > 20 and len(libs) > 20
+    assert not named - set(read.findall(src)), sorted(named - set(read.findall(src)))
+    assert not libs - named, sorted(libs - named)
 
 
 def test_no_switch_makes_a_result_wrong():
