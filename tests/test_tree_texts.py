@@ -98,3 +98,13 @@ def test_no_device_source_ends_the_process():
             if re.search(r"\b(_exit|_Exit|quick_exit|exit|abort)\s*\(", re.sub(r"//[^\n]*", "", text)):
                 bad.append(path)
     assert not bad, bad
+
+
+def test_hip_sources_are_compiled_without_packed_fp32():
+    with open(os.path.join(ROOT, "nextpolish_amd", "csrc", "Makefile")) as f:
+        text = f.read()
+    flags = re.search(r"^HIPFLAGS *:=(.*)$", text, re.M).group(1)
+    assert "-Xclang -target-feature -Xclang -packed-fp32-ops" in flags
+    assert re.search(r"\$\(HIPCC\) \$\(HIPFLAGS\) -c", text) and len(re.findall(r"\$\(HIPCC\)[^\n]* -c ", text)) == 1
+    bad = [path for path, body in texts() if path.startswith("nextpolish_amd") and re.search(r"v_pk_(add|mul|fma)_f32", body)]
+    assert not bad, bad
