@@ -274,7 +274,7 @@ def lgs_roofline(worker_code, env, alg_bytes, with_pmc):
     return out
 
 
-def lgs_leg(rank, local_rank, workers, contig_mb, calls, with_ref, with_pmc):
+def lgs_leg(rank, local_rank, workers, contig_mb, calls, with_ref, with_pmc, threads=3):
     """Long-read path (BASELINE configs[3] shape: 20x ONT-like reads, lib/nextpolish2.so ctg_cns_core, BAM -> consensus):
     `workers` worker processes share this rank's GPU (the reference's -p model), each polishes its contig `calls`
     times after a warm-up; rate = polished bp of all workers / span from the common start to the last end."""
@@ -290,7 +290,7 @@ def lgs_leg(rank, local_rank, workers, contig_mb, calls, with_ref, with_pmc):
         f.write(bam + "\n")
     go = os.path.join(d, "go")
     env = dict(os.environ, NP2_DEVICE=str(local_rank))
-    wt = os.environ.get("NP2_WORKER_THREADS", "2")   # many workers share the host cores of one GPU
+    wt = os.environ.get("NP2_WORKER_THREADS", str(threads))   # 14 workers on 16 cores: 108 Mbp/s with 2 threads each, 118 with 3, 114 with 4
     env["NP_HOST_THREADS"] = wt
     env["NP_IO_THREADS"] = wt
     lib2 = os.path.join(ROOT, "nextpolish_amd", "lib", "nextpolish2.so")
@@ -659,7 +659,7 @@ def main():
     ap.add_argument("--pmc-batches", type=int, default=4, help="batches of the workload the two rocprofv3 --pmc child runs polish (generating all 600 M records twice more is most of a full-size run)")
     ap.add_argument("--no-e2e", action="store_true", help="skip the from-files leg")
     ap.add_argument("--no-lgs", action="store_true", help="skip the long-read (nextpolish2) leg")
-    ap.add_argument("--lgs-workers", type=int, default=14, help="worker processes per GPU of the long-read leg (x NP2_WORKER_THREADS host threads each, default 2); with this process and its helpers at most 16 processes share a card")
+    ap.add_argument("--lgs-workers", type=int, default=14, help="worker processes per GPU of the long-read leg (x NP2_WORKER_THREADS host threads each, default 3, 2 when ranks share the host); with this process and its helpers at most 16 processes share a card")
     ap.add_argument("--lgs-mb", type=float, default=5.0, help="contig length (Mb) each long-read worker polishes")
     ap.add_argument("--lgs-calls", type=int, default=24, help="timed calls per long-read worker (the rate is bp over the span from the common start to the last end; measured: 0.63 s of ramp and stragglers + 0.70 s per round of calls, so 4 / 8 calls read 140 / 154 Mbp/s of a steady state of 171: a worker of a real run polishes hundreds of windows)")
     ap.add_argument("--no-lgs-config4", action="store_true", help="skip the 100 Mb / 67-contig long-read run (BASELINE configs[3] at its stated size)")
@@ -834,13 +834,14 @@ def main():
         if world > 1:
             dist.barrier()
         lgs_workers = args.lgs_workers if world == 1 else max(2, min(args.lgs_workers, (ncpu * 3 // 4) // world))   # the ranks share the host cores
+        lgs_threads = int(os.environ.get("NP2_WORKER_THREADS", "3" if world == 1 else "2"))
         lgs = lgs_leg(rank, local_rank, lgs_workers, args.lgs_mb, args.lgs_calls,
-                      rank == 0 and world == 1 and not args.no_cpu_baseline, rank == 0 and world == 1 and not args.no_pmc)
+                      rank == 0 and world == 1 and not args.no_cpu_baseline, rank == 0 and world == 1 and not args.no_pmc, lgs_threads)
         if world == 1 and rank == 0 and "error" not in lgs:
             # the same leg on the host budget of one rank of eight (this box's cores / 8): does the feed of one GPU still hold?
             bt = max(2, ncpu // 8)
             wt = int(os.environ.get("NP2_WORKER_THREADS", "2"))
-            l8 = lgs_leg(1, local_rank, max(1, bt // wt), args.lgs_mb, max(2, args.lgs_calls // 4), False, False)
+            l8 = lgs_leg(1, local_rank, max(1, bt // wt), args.lgs_mb, max(2, args.lgs_calls // 4), False, False, wt)
             if "error" not in l8:
                 v8 = l8["bp"] / 1e6 / l8["seconds"]
                 lgs["at_8_rank_budget"] = {"host_threads": bt, "workers": l8["workers"], "mbp_s": round(v8, 2),
@@ -918,7 +919,7 @@ def main():
                 out["lgs"] = {"metric": "polished Mbp/s (ctg_cns_core, long reads, sorted BAM in the page cache -> consensus, warm workers)",
                               "value": round(lgs["bp"] / 1e6 / lgs["seconds"], 3), "unit": "Mbp/s", "n_gpus": world,
                               "config": {"workload": "%.1f Mb synthetic contig + 20x ONT-like reads (8 kb, 7%% errors) per worker, %d worker processes per GPU, "
-                                                     "%d calls each, %s host threads per worker" % (args.lgs_mb, lgs["workers"], args.lgs_calls, os.environ.get("NP2_WORKER_THREADS", "2"))},
+                                                     "%d calls each, %s host threads per worker" % (args.lgs_mb, lgs["workers"], args.lgs_calls, lgs_threads)},
                               "s_per_call": lgs["s_per_call"], "host_cpu_s_per_mbp": lgs["cpu_s_per_mbp"]}
                 for k in ("roofline", "cpu_baseline", "config4", "at_8_rank_budget"):
                     if k in lgs:
