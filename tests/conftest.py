@@ -140,9 +140,10 @@ def pytest_runtest_logfinish(nodeid, location):
 
 @pytest.fixture(scope="session", autouse=True)
 def _built():
-    """Build the in-tree libraries once per session (no-op when up to date)."""
+    """The in-tree libraries as they were built; built once if they are not there.  After a change to a source: __graft_entry__.build()."""
     import __graft_entry__ as g
-    g.build()
+    if not g.is_built():
+        g.build()
 
 
 def ref_binary():
