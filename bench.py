@@ -1,13 +1,12 @@
 #!/usr/bin/env python
-"""Headline benchmark: short-read score_chain polishing throughput (BASELINE.json metric) on the metric's own configuration.
+"""Headline benchmark: short-read score_chain polishing throughput on a 3 Gb draft at 30x.
 
-Workload (default c5_3gb_30x = the configuration BASELINE.json's metric is quoted on: a 3 Gb human-scale draft at 30x; it fits one
-MI355X): a FIXED synthetic draft (contig lengths log-uniform, SURVEY.md 8d) + 30x simulated 2x150 bp PE reads = 600 M records.
+Workload (default c5_3gb_30x: a 3 Gb human-scale draft at 30x; it fits one
+MI355X): a FIXED synthetic draft (contig lengths log-uniform) + 30x simulated 2x150 bp PE reads = 600 M records.
 The contigs are dealt longest-first over the N ranks (contigs are independent units: strong scaling of one fixed draft, no
 data-path collective; reference: source/lib/nextpolish1.py:181-189,223-224) and packed into batches of <= 260 Mb.
 
-One "step" = one full score_chain pass over the WHOLE draft with every record batch RESIDENT IN HBM when the timed region starts
-(SURVEY.md 8d's timing scope 1; since round 6 -- rounds 1-5 timed the PCIe-inclusive pass and reported the resident one beside it):
+One "step" = one full score_chain pass over the WHOLE draft with every record batch RESIDENT IN HBM when the timed region starts:
 every kernel of np1_device.hip's launch sequence over all batches on the device lanes (`value`).  Beside it, in the same JSON line:
   streamed          the PCIe-inclusive rate of the same pass: decoded records in pinned host memory -> async H2D -> kernels -> D2H of the
                     polished strings, double-buffered on the lanes (bound by the H2D of the record stream; never `value`)
@@ -17,7 +16,7 @@ every kernel of np1_device.hip's launch sequence over all batches on the device 
   parity            contigs of this very run compared with the CPU oracle (md5 of the polished strings)
   roofline          dominant kernel: algorithmic bytes per launch / HIP-event time per launch vs the 8 TB/s HBM peak, and
                     the PMC traffic per launch (two rocprofv3 --pmc passes)
-  cpu_baseline      the compiled reference (oracle/_ref/nextpolish1) on this box's host cores, one process per core like -p N,
+  cpu_baseline      the compiled reference (oracle/_ref/nextpolish1) on this host's cores, one process per core like -p N,
                     and one core alone, on a bounded sample of the same shape (rank 0, N=1 only)
   lgs               the long-read path (lib/nextpolish2.so ctg_cns_core) with its own roofline and cpu_baseline
   snp_phase         task 3 (np1_batch_snp_phase): diploid draft, short + long reads resident in HBM, with the compiled reference beside it (N=1 only)
@@ -39,7 +38,7 @@ sys.path.insert(0, ROOT)
 
 HBM_PEAK_GBS = 8000.0   # /opt/skills/guides/MI355X_MICROARCH.md: HBM3E 8 TB/s spec
 WORKLOADS = {
-    # name: (total draft bp, depth, min contig, max contig, batch bp)      -- SURVEY.md 8d synthetic shapes
+    # name: (total draft bp, depth, min contig, max contig, batch bp)
     "c3_100mb_30x": (100000000, 30.0, 50e3, 5e6, 13000000),
     "c2_5mb_50x": (5000000, 50.0, 1e6, 2.5e6, 13000000),
     "c5_3gb_30x": (3000000000, 30.0, 2e6, 250e6, 260000000),
@@ -70,7 +69,7 @@ def contig_lengths(total, lo, hi, seed=20250117 + 3):
 
 def host_cores():
     n = len(os.sched_getaffinity(0))
-    try:   # cgroup v2 CPU quota, when the box has one
+    try:   # cgroup v2 CPU quota, when there is one
         q, p = open("/sys/fs/cgroup/cpu.max").read().split()
         if q != "max":
             n = min(n, max(1, int(int(q) / int(p))))
@@ -275,14 +274,14 @@ def lgs_roofline(worker_code, env, alg_bytes, with_pmc):
 
 
 def lgs_leg(rank, local_rank, workers, contig_mb, calls, with_ref, with_pmc, threads=3):
-    """Long-read path (BASELINE configs[3] shape: 20x ONT-like reads, lib/nextpolish2.so ctg_cns_core, BAM -> consensus):
+    """Long-read path (20x ONT-like reads, lib/nextpolish2.so ctg_cns_core, BAM -> consensus):
     `workers` worker processes share this rank's GPU (the reference's -p model), each polishes its contig `calls`
     times after a warm-up; rate = polished bp of all workers / span from the common start to the last end."""
     from nextpolish_amd import _native as nat
     d = tempfile.mkdtemp(prefix="np2bench_r%d_" % rank)
     L = int(contig_mb * 1e6)
     st = nat.Stream.synth_long([L], depth=20.0, seed=9000 + rank)
-    alg_bytes = st.algorithmic_bytes(False) - L + (L + 3) // 4 + L    # records + 2-bit draft + polished string (SURVEY.md 8d, path B)
+    alg_bytes = st.algorithmic_bytes(False) - L + (L + 3) // 4 + L    # records + 2-bit draft + polished string
     fa, bam, fofn = os.path.join(d, "g.fa"), os.path.join(d, "r.bam"), os.path.join(d, "bam.fofn")
     st.write_files(fa, bam)
     st.close()
@@ -542,7 +541,7 @@ def _time_files(fa, bam, draft_bp, threads, n_records, cold_runs, warm_runs, pip
                        "what": "md5 of the contigs the oracle was run on (the streamed passes' parity set), as they left np1_pipe_run_files in the first warm pass: "
                                "BAM + FASTA on disk -> device inflate + CRC + record split + kernels"}
     if stats[4] > 0 and stats[0] > 0:
-        # the dominant kernel of the from-files leg (VERDICT r4 weak 6): the BGZF block decoder.  Algorithmic bytes of one launch = the compressed
+        # the dominant kernel of the from-files leg: the BGZF block decoder.  Algorithmic bytes of one launch = the compressed
         # bytes it reads + the inflated bytes it writes; time = HIP events around the launch on the lane's stream (np1_ingest.hip), warm passes only
         algo = (stats[2] + stats[3]) / stats[4]
         ms = stats[0] / stats[4]
@@ -562,17 +561,17 @@ def e2e_from_files(streams, draft_bp, threads, n_records, expect=None):
     from nextpolish_amd.device import Pipe
     d = tempfile.mkdtemp(prefix="np1e2e_")
     out = {}
-    pipe = Pipe(int(os.environ.get("LOCAL_RANK", "0")), lanes=int(os.environ.get("NP1_E2E_LANES", "3")))      # round-4 sweep (tests/tools/r4_e2e_lanes.py): 3 > 2 > 4
+    pipe = Pipe(int(os.environ.get("LOCAL_RANK", "0")), lanes=int(os.environ.get("NP1_E2E_LANES", "3")))      # measured with tests/tools/r4_e2e_lanes.py: 3 > 2 > 4
     try:
         fa, bam = os.path.join(d, "g.fa"), os.path.join(d, "r.bam")
         t_write = _write_files(streams, fa, bam, 1)
         full = _time_files(fa, bam, draft_bp, threads, n_records, 2, 2, pipe, expect=expect)
         full["qualities"] = "Illumina-like, binned (2/12/23/37; ~93 % in the top bin), BGZF level 1"
         full["write_seconds"] = round(t_write, 1)
-        bt = max(1, threads // 8)      # what a rank gets of this box's cores when eight ranks share them
+        bt = max(1, threads // 8)      # what a rank gets of this host's cores when eight ranks share them
         b8 = _time_files(fa, bam, draft_bp, bt, n_records, 1, 0, None)
         full["at_8_rank_budget"] = {"host_threads": bt, "mbp_s": b8["mbp_s"], "seconds": b8["seconds"], "fraction_of_full_budget": round(b8["mbp_s"] / max(1e-9, full["mbp_s"]), 3),
-                                    "what": "the cold CLI run again with NP_IO_THREADS = this box's cores / 8"}
+                                    "what": "the cold CLI run again with NP_IO_THREADS = this host's cores / 8"}
         full["what"] = ("cold: nextpolish1 scorechain g.fa r.bam > out.fa, new process each time (HIP start-up and first-touch allocations inside), "
                         "best of 2, files in the page cache, %d host threads; warm: the same files through np1_pipe_run_files of a running "
                         "process (device BGZF inflate + CRC + record split + kernels + D2H), best of 2 after one pass" % threads)
@@ -638,7 +637,7 @@ def parity_check(pipe, streams, budget_bp, per_batch_cap_bp=40000000, big_second
     return {"oracle_md5": oracle_md5, "contigs": len(chosen), "draft_bp": sum(x[0] for x in chosen), "batches_represented": len({k for _, k, _ in chosen}), "batches": len(streams),
             "batches_unchecked": unchecked, "identical": not bad, "differing": bad, "oracle_seconds": round(time.time() - t0, 1),
             "what": "md5 of the polished strings of the timed streamed passes vs oracle/np1_oracle (CPU restatement): the shortest contigs of the draft and "
-                    "the shortest contig of every batch (up to %d Mb each, or whatever the oracle walks in %d s on one core: VERDICT r4 weak 3)" % (per_batch_cap_bp // 1000000, int(big_seconds))}
+                    "the shortest contig of every batch (up to %d Mb each, or whatever the oracle walks in %d s on one core)" % (per_batch_cap_bp // 1000000, int(big_seconds))}
 
 
 def main():
@@ -662,7 +661,7 @@ def main():
     ap.add_argument("--lgs-workers", type=int, default=14, help="worker processes per GPU of the long-read leg (x NP2_WORKER_THREADS host threads each, default 3, 2 when ranks share the host); with this process and its helpers at most 16 processes share a card")
     ap.add_argument("--lgs-mb", type=float, default=5.0, help="contig length (Mb) each long-read worker polishes")
     ap.add_argument("--lgs-calls", type=int, default=24, help="timed calls per long-read worker (the rate is bp over the span from the common start to the last end; measured: 0.63 s of ramp and stragglers + 0.70 s per round of calls, so 4 / 8 calls read 140 / 154 Mbp/s of a steady state of 171: a worker of a real run polishes hundreds of windows)")
-    ap.add_argument("--no-lgs-config4", action="store_true", help="skip the 100 Mb / 67-contig long-read run (BASELINE configs[3] at its stated size)")
+    ap.add_argument("--no-lgs-config4", action="store_true", help="skip the 100 Mb / 67-contig long-read run")
     ap.add_argument("--no-phase", action="store_true", help="skip the snp_phase (task 3) leg")
     ap.add_argument("--phase-mb", type=float, default=20.0, help="draft length (Mb) of the snp_phase leg")
     args = ap.parse_args()
@@ -670,7 +669,7 @@ def main():
     rank = int(os.environ.get("RANK", "0"))
     local_rank = int(os.environ.get("LOCAL_RANK", "0"))
     world = int(os.environ.get("WORLD_SIZE", "1"))
-    # host threads of this rank = the box's cores / ranks (generator, BAM writer, loaders; read once when the library loads)
+    # host threads of this rank = the host's cores / ranks (generator, BAM writer, loaders; read once when the library loads)
     per_rank = max(1, host_cores() // max(1, world))
     os.environ.setdefault("NP_HOST_THREADS", str(per_rank))
     os.environ.setdefault("NP_IO_THREADS", str(per_rank))
@@ -716,7 +715,7 @@ def main():
     t_gen = time.time() - t_gen
     n_reads = sum(s.n_reads for s in streams)
     alg_in = [s.algorithmic_bytes(False) for s in streams]   # records (32 + 4 n_cigar + ceil(l/2)) + draft, per batch
-    # The upload forms (2-bit bases, compact record fields: DESIGN.md section 4) are built ONCE per stream on the host, outside the timed
+    # The upload forms (2-bit bases, compact record fields: np1_upload.h) are built ONCE per stream on the host, outside the timed
     # steps; a stream that is polished once pays for them once.  Timed here and reported next to `value` (upload_forms_build_s,
     # streamed_single_use) so that the line says what its scope leaves out.
     L0 = nat.lib()
@@ -780,7 +779,7 @@ def main():
     parity = parity_check(pipe, streams, int(args.parity_mb * 1e6), big_seconds=args.parity_big_seconds) if rank == 0 else None
     streamed_lengths = pipe.result_lengths(streams)
 
-    # ---- the timed steps (SURVEY 8d scope 1): every batch of the rank's share of the draft resident in HBM when the clock starts; a step = one
+    # ---- the timed steps: every batch of the rank's share of the draft resident in HBM when the clock starts; a step = one
     # score_chain pass over all of them on the lanes (no H2D / D2H inside).  W untimed steps, then exactly K between two barriers.
     if L.np1_pipe_upload(pipe.handle, harr, len(streams)) != 0:
         raise SystemExit("upload: " + nat.last_error())
@@ -838,7 +837,7 @@ def main():
         lgs = lgs_leg(rank, local_rank, lgs_workers, args.lgs_mb, args.lgs_calls,
                       rank == 0 and world == 1 and not args.no_cpu_baseline, rank == 0 and world == 1 and not args.no_pmc, lgs_threads)
         if world == 1 and rank == 0 and "error" not in lgs:
-            # the same leg on the host budget of one rank of eight (this box's cores / 8): does the feed of one GPU still hold?
+            # the same leg on the host budget of one rank of eight (this host's cores / 8): does the feed of one GPU still hold?
             bt = max(2, ncpu // 8)
             wt = int(os.environ.get("NP2_WORKER_THREADS", "2"))
             l8 = lgs_leg(1, local_rank, max(1, bt // wt), args.lgs_mb, max(2, args.lgs_calls // 4), False, False, wt)
@@ -846,9 +845,9 @@ def main():
                 v8 = l8["bp"] / 1e6 / l8["seconds"]
                 lgs["at_8_rank_budget"] = {"host_threads": bt, "workers": l8["workers"], "mbp_s": round(v8, 2),
                                            "fraction_of_full_budget": round(v8 / max(1e-9, lgs["bp"] / 1e6 / lgs["seconds"]), 3),
-                                           "what": "workers x threads limited to this box's cores / 8, as when eight ranks share the host"}
+                                           "what": "workers x threads limited to this host's cores / 8, as when eight ranks share the host"}
         if world == 1 and rank == 0 and "error" not in lgs and not args.no_lgs_config4:
-            # BASELINE configs[3] at its stated size: ~100 Mb in 67 contigs (four of them two or three windows), 20x ONT-like reads, the contigs
+            # ~100 Mb in 67 contigs (four of them two or three windows), 20x ONT-like reads, the contigs
             # in 8 groups (one FASTA + BAM each) taken by worker processes like the reference's -p model: from cold processes to the last
             # consensus, every contig compared with the md5 the compiled reference produced (tests/tools/check_config4.py, tests/golden/)
             env4 = dict(os.environ, NP2_DEVICE=str(local_rank), NP_HOST_THREADS=os.environ.get("NP2_WORKER_THREADS", "2"), NP_IO_THREADS=os.environ.get("NP2_WORKER_THREADS", "2"))
@@ -858,7 +857,7 @@ def main():
                 c4 = json.loads(q.stdout.strip().splitlines()[-1])
                 lgs["config4"] = {"mbp_s": c4.get("mbp_s"), "draft_bp": c4.get("draft_bp"), "contigs": c4.get("contigs"), "groups": c4.get("groups"), "procs": c4.get("procs"),
                                   "polish_s": c4.get("polish_s"), "mismatches_vs_reference_golden": c4.get("mismatches"), "missing": c4.get("missing"),
-                                  "what": "100 Mb / 67 contigs / 20x ONT-like (BASELINE configs[3]), 8 cold worker processes sharing the GPU, process start and "
+                                  "what": "100 Mb / 67 contigs / 20x ONT-like, 8 cold worker processes sharing the GPU, process start and "
                                           "first allocations included; every contig's md5 against the compiled reference's"}
             except Exception as e:      # noqa: BLE001
                 lgs["config4"] = {"error": (q.stderr or str(e))[-300:]}

@@ -98,7 +98,7 @@ void polishresult_destory(PolishResult* polishresult);
 
 const char* np1_last_error(void);
 
-/* Host-side decoded record stream = whole contigs + their BAM records (see DESIGN.md "data layout"). */
+/* Host-side decoded record stream = whole contigs + their BAM records. */
 typedef struct np1_stream np1_stream;
 
 typedef struct {
@@ -148,7 +148,7 @@ int np1_streams_write_files(np1_stream* const* streams, int n, const char* fasta
 int np1_streams_write_files_q(np1_stream* const* streams, int n, const char* fasta, const char* bam, int bgzf_level, int qual_model);
 void np1_stream_free(np1_stream* s);
 
-/* Synthetic workload (SURVEY.md §8d).  Field meanings: nextpolish_amd/csrc/np_synth.h */
+/* Synthetic workload.  Field meanings: nextpolish_amd/csrc/np_synth.h */
 typedef struct {
     uint64_t seed;
     int32_t n_contigs;
@@ -213,10 +213,10 @@ np1_batch* np1_batch_upload(np1_ctx* ctx, const np1_stream* s);
 void np1_batch_free(np1_batch* b);
 /* Streaming use: an empty batch object bound to a context, (re)filled from successive host streams.  Its HBM buffers only
  * grow, so nothing is allocated in steady state; np1_batch_reload leaves the H2D copies in flight on the context's stream.
- * Round 5: the bytes of an UNPINNED stream are taken while the call runs (through the library's own pinned ring: the stream may be freed
+ * The bytes of an UNPINNED stream are taken while the call runs (through the library's own pinned ring: the stream may be freed
  * right after); np1_stream_pin copies the arrays an upload moves into one page-locked arena of the stream, from which the copies run
  * asynchronously at full PCIe rate (the stream must then outlive the pass; np1_stream_free waits for the device).  The GPU never reads
- * the caller's pageable memory in place (csrc/np_hostcopy.h, DESIGN.md section 12).  np1_batch_results_fetch moves the polished strings of the whole batch into a pinned host buffer with one D2H
+ * the caller's pageable memory in place (csrc/np_hostcopy.h).  np1_batch_results_fetch moves the polished strings of the whole batch into a pinned host buffer with one D2H
  * copy on the same stream and waits for it; np1_batch_results_ptr()[bounds[c] .. bounds[c+1]) is contig c. */
 np1_batch* np1_batch_create(np1_ctx* ctx);
 int np1_batch_reload(np1_batch* b, const np1_stream* s);
@@ -227,7 +227,7 @@ int np1_batch_results_fetch(np1_batch* b);
 const char* np1_batch_results_ptr(np1_batch* b);
 const uint32_t* np1_batch_results_bounds(np1_batch* b);
 
-/* Streamed polishing (SURVEY.md 8d timing scope 1): batches flow  pinned host arrays -> H2D -> score_chain kernels -> D2H
+/* Streamed polishing: batches flow  pinned host arrays -> H2D -> score_chain kernels -> D2H
  * on `lanes` device lanes (one HIP stream + one reusable HBM batch + one host thread each), so the copies of one batch
  * overlap the kernels of another.  np1_pipe_run polishes the given streams (batch k = streams[k]) and keeps the polished
  * strings inside the pipe until the next run: np1_pipe_result(p, k, c, &len) is contig c of batch k.
@@ -280,9 +280,9 @@ int np1_batch_score_chain(np1_batch* b, const Configure* cfg, float* stage_ms);
 int np1_batch_kmer_count(np1_batch* b, const Configure* cfg, float* stage_ms);
 /* Makes np1_batch_kmer_count of this batch replay the reference's region iterator (reference: source/lib/contig.c:982-1043 over htslib's
  * hts_itr_query / hts_itr_next): per part the records the first loop of ss_kmer_correct gets, the record left in its buffer and the
- * passes of the second loop come from the BAM index and the records' virtual offsets instead of "records in file order" (DESIGN.md
- * section 3).  `s` = the stream the batch was uploaded from, read from `bam` (np1_stream_load); it has to stay alive until the pass is
- * done.  Experimental in round 2: equal to the compiled reference through the host model, not yet validated on a GPU. */
+ * passes of the second loop come from the BAM index and the records' virtual offsets instead of "records in file order".
+ * `s` = the stream the batch was uploaded from, read from `bam` (np1_stream_load); it has to stay alive until the pass is
+ * done. */
 int np1_batch_enable_replay(np1_batch* b, const np1_stream* s, const char* bam);
 /* task 4 on an uploaded batch (reference: source/lib/snpvalid.c:3-36 snp_valid; needs a stream loaded with qualities) */
 int np1_batch_snp_valid(np1_batch* b, const Configure* cfg, float* stage_ms);
@@ -291,14 +291,14 @@ int np1_batch_snp_valid(np1_batch* b, const Configure* cfg, float* stage_ms);
  * same context.  cfg->read_len / read_tlen as config_init sets them.  The result lands in `sr` (np1_batch_result_*).  Inputs for
  * which the reference itself reads through a null or unset pointer fail with an error message instead of a result. */
 int np1_batch_snp_phase(np1_batch* sr, np1_batch* lr, const Configure* cfg);
-/* Intra-contig tiling (np1_tile.cpp): one contig of any length polished as independent tiles of tile_bp draft bases with
+/* Intra-contig tiling (csrc/np1_tile.cpp): one contig of any length polished as independent tiles of tile_bp draft bases with
  * a halo of halo_bp on each side, each tile reading its own region of the BAM through the index; the join is exact (a tile is redone
  * with a doubled halo when a halo holds no slot the chain restarts behind).  The reference takes contigs up to 2^31 bases
  * (source/nextPolish:101-102) in one score_chain call (source/lib/scorechain.c:3-15); this is that call for contigs beyond one HBM batch.
  * first_tile / tile_stride: this call polishes tiles first_tile, first_tile + tile_stride, ... and returns their pieces concatenated in
  * tile order (0, 1: all of them = the polished contig).  Tiles are independent, so the tiles of one dominant contig can be dealt over
  * ranks: a call with first_tile = k and a stride of at least the number of tiles returns the piece of tile k alone, and the pieces of all
- * tiles in tile order are the polished contig (the callers of this repository still deal whole contigs over ranks: DESIGN.md section 11).
+ * tiles in tile order are the polished contig.
  * *out: malloc'd, NUL-terminated (np1_free_string).
  * stats (optional, 4 words): tiles, tiles recomputed with a wider halo, records read, records of the largest tile.
  * Pieces: np1_batch_keep_single (before the run) makes a one-contig batch remember which slots left the vote with one state;

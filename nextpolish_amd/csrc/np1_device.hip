@@ -144,7 +144,7 @@ static void stream_facts(np1_stream* st) {
         st->ncig16.resize(n);
         for (size_t i = 0; i < n; ++i) st->ncig16[i] = (uint16_t)s.n_cigar[i];
     }
-    // ---- the upload forms (np1_upload.h; DESIGN.md section 4)
+    // ---- the upload forms (np1_upload.h)
     static const bool full = getenv("NP1_UPLOAD") && strcmp(getenv("NP1_UPLOAD"), "full") == 0;
     const size_t nb = s.seq.size();
     st->seq2.clear(); st->esc_at.clear(); st->esc_val.clear();
@@ -588,9 +588,9 @@ int np1_batch_score_chain(np1_batch* b, const Configure* cfg, float* stage_ms) {
             };
             HIPCHK(hipMemsetAsync(&totals[8], 0, 8 * POOL_SHARDS, q));
             t0(5);
-            // Default: k_tile3.  NP1_TILE=9: k_tile9 (np1_tile9.h; round 4: four slots per lane, agreeing records counted per window), k_tile3
+            // Default: k_tile3.  NP1_TILE=9: k_tile9 (np1_tile9.h: four slots per lane, agreeing records counted per window), k_tile3
             // for the chunks it hands back -- exact (GPU-tested in a subprocess: tests/test_gpu_score_chain.py) but slower on MI355X as it stands
-            // (DESIGN.md section 7 has its phase clocks).  The general-rate fp64 path spills a record for every slot and stays with k_tile3.
+            // (NP1_T9_PHASES=1 prints its phase clocks).  The general-rate fp64 path spills a record for every slot and stays with k_tile3.
             static const int tile_kind_env = getenv("NP1_TILE") ? atoi(getenv("NP1_TILE")) : 3;
             const int tile_kind = fp_rate ? 3 : tile_kind_env;
             const uint32_t heads_cap5 = (uint32_t)std::min<size_t>(b->heads.cap / 4, 0xfffffff0u);
@@ -1133,7 +1133,7 @@ int np1_batch_result_copy(np1_batch* b, int64_t c, char* dst, int64_t cap) {
     return 0;
 }
 
-// ---- intra-contig tiling (np1_tile.cpp; DESIGN.md section 8) -------------------------------------------------------------------------
+// ---- intra-contig tiling (np1_tile.cpp) -------------------------------------------------------------------------
 extern "C" int np1_batch_keep_single(np1_batch* b, int on) {
     if (!b) { np1_set_error("np1_batch_keep_single: null batch"); return -1; }
     b->keep_single = on != 0;

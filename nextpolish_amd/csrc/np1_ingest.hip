@@ -81,7 +81,7 @@ __global__ __launch_bounds__(64, 4) void k_inflate_lanes(const uint8_t* __restri
     }
 }
 
-// Lane-per-block decoder with its primary tables in LDS (np_inflate_lds.h; round 6): a workgroup is one wave, every lane inflates blocks of
+// Lane-per-block decoder with its primary tables in LDS (np_inflate_lds.h): a workgroup is one wave, every lane inflates blocks of
 // its own (lane, lane + lanes, ...); 2^LB + 2^DB 16-bit slots per lane, [slot][lane], fill the LDS of a CU with one wave (10 / 8 bits:
 // exactly 160 KiB) or two (9 / 6 bits: 72 KiB each).  The grid is as many waves as the chip holds at once.
 struct LdsTab {
@@ -258,7 +258,7 @@ struct ScatterOut {
     uint32_t* cigar; uint8_t* seq; uint8_t* mapq; int32_t* isize; uint64_t* qualoff; uint8_t* qual;
 };
 
-// n bytes between two byte-aligned places, 16 at a time (round 6: word loads and BYTE stores before -- 75 store instructions per record, every one
+// n bytes between two byte-aligned places, 16 at a time (word loads and byte stores were 75 store instructions per record, every one
 // a transaction per lane; global loads and stores of any width take any alignment on this device, as the block decoder's do)
 struct __attribute__((packed, aligned(1))) Bytes16 { uint64_t a, b; };
 __device__ __forceinline__ void copy_unaligned(uint8_t* __restrict__ dst, const uint8_t* __restrict__ src, uint32_t n) {
@@ -393,9 +393,9 @@ struct HostBuf {
 struct FileRun { uint64_t coff, bytes, comp_at, last_block; };   // last_block: highest file offset at which a needed block may start
 
 struct Staging::Impl {
-    // Round 6: the compressed bytes of a batch are no longer copied into pinned memory of the staging object.  The cold start of the
+    // The compressed bytes of a batch are not copied into pinned memory of the staging object.  With such copies the cold start of the
     // from-files CLI was page-locking: a staging object grew to the compressed size of the largest batch it met (2.2 GB for a 250 Mb contig
-    // at 30x) at ~1.6 GB/s of hipHostMalloc, every loader thread its own, every growth from scratch -- 5 of the 8 s of a 3 Gb run.  Now
+    // at 30x) at ~1.6 GB/s of hipHostMalloc, every loader thread its own, every growth from scratch -- 5 of the 8 s of a 3 Gb run.  So
     // prepare() walks the BGZF headers in the mapped file (no bulk read), and ingest() sends the runs to the device through the small ring
     // of pinned slots every large pageable copy already uses (np_hostcopy.h): pread() straight into a slot on the helper threads, DMA out.
     const BamSource* src = nullptr;
@@ -669,8 +669,8 @@ int ingest(np1_batch* b, Staging* st, bool with_qual, Scratch* scr, const np::Ba
     uint64_t* d_tot = reinterpret_cast<uint64_t*>(W.small.as<uint8_t>() + 64);   // scan totals
     uint64_t n_rec = 0;
     if (n_blocks) {
-        // which decoder: a lane per block with its tables in LDS (np_inflate_lds.h; round 6: 7 / 5-bit primaries, three waves per CU -- measured
-        // 14.4 ms for 34 k blocks, 45.5 ms for 138 k, against 42.6 / 94.8 ms of the round-4 lane decoder: profiles/r6_inflate_lds.txt) when the
+        // which decoder: a lane per block with its tables in LDS (np_inflate_lds.h; 7 / 5-bit primaries, three waves per CU -- measured
+        // 14.4 ms for 34 k blocks, 45.5 ms for 138 k, against 42.6 / 94.8 ms of the lane decoder with its tables in HBM: profiles/r6_inflate_lds.txt) when the
         // batch has blocks enough to fill the chip with lanes, else a wave per block (np_inflate_dev.h).
         // NP1_INFLATE=lds<LB><DB> | lanes (np_inflate_lane.h, tables in HBM) | wave forces one.
         static const int mode = [] {

@@ -54,7 +54,7 @@ int launch_tile3(hipStream_t st, int level, const ReadsDev& R, const uint32_t* s
                  uint16_t* slot_res, uint32_t* slot_rec, uint32_t* pool, uint32_t pool_cap, uint32_t* counters,
                  uint32_t* heads, uint32_t heads_cap, uint32_t* redo_out, uint32_t redo_ci, uint32_t flag_single,
                  unsigned long long* votes);
-// k_tile9 (default since round 4, np1_tile9.h): four slots per lane, agreeing records counted per window, the rest deferred and tallied in
+// k_tile9 (NP1_TILE=9, np1_tile9.h): four slots per lane, agreeing records counted per window, the rest deferred and tallied in
 // record order; the vote chunks of a wave that runs out of room land in redo_out for launch_tile3(level 1)
 int launch_tile9(hipStream_t st, const ReadsDev& R, const uint32_t* soff, const uint32_t* desc, const uint32_t* ovf_pool, const uint32_t* chunk_first,
                  const uint32_t* chunk_last, uint32_t n_chunks, const uint8_t* slot_info, const uint32_t* slot_g, uint32_t S, uint32_t max_lq,

@@ -2,7 +2,7 @@
 //
 // The reference walks every read twice through htslib and keeps, per draft base, malloc'd lists of
 // (3-base context, count) pairs, then runs a sequential fp64 chain DP over the whole contig
-// (reference: source/lib/contig.c:170-496, SURVEY.md appendix A).  Here the same result is produced by
+// (reference: source/lib/contig.c:170-496).  Here the same result is produced by
 // data-parallel stages over a decoded record stream resident in HBM:
 //
 //   k_prep      1 lane / record : filter, trimmed query window, insertion-column max-reduce   (contig.c:202-245,333-358,667-677)
@@ -16,7 +16,7 @@
 //   k_fixfirst  reference quirk: base 0 of a contig keeps its input state when it owns insertion columns
 //   scan+k_emit polished characters, lowercase mask with the carried "sign"                       (contig.c:736-786)
 //
-// Integer / byte work throughout: no MFMA.  Bound: HBM bytes of the record stream (SURVEY.md §8d).
+// Integer / byte work throughout: no MFMA.  Bound: HBM bytes of the record stream.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <stdlib.h>
@@ -112,8 +112,8 @@ __global__ __launch_bounds__(SCAN_T) void k_scan_final(F f, uint64_t n, const ui
                                                        OutT* __restrict__ out, const uint64_t* __restrict__ total) {
     __shared__ uint64_t sh[SCAN_T];
     uint64_t base = (uint64_t)blockIdx.x * SCAN_TILE;
-    // thread t owns SCAN_ITEMS consecutive elements; they come in COALESCED through a padded tile in LDS (round 6: read from its own 64 bytes,
-    // every load instruction of a wave touched 64 different lines; every element of every scan of this file is below 2^32)
+    // thread t owns SCAN_ITEMS consecutive elements; they come in COALESCED through a padded tile in LDS (read from its own 64 bytes,
+    // every load instruction of a wave would touch 64 different lines; every element of every scan of this file is below 2^32)
     __shared__ uint32_t tile[SCAN_TILE + SCAN_TILE / 32];
     uint64_t first = base + (uint64_t)threadIdx.x * SCAN_ITEMS;
     uint64_t v[SCAN_ITEMS];
@@ -141,8 +141,8 @@ __global__ __launch_bounds__(SCAN_T) void k_scan_final(F f, uint64_t n, const ui
     }
     uint64_t run = tile_offs[blockIdx.x] + sh[threadIdx.x] - acc;
     if constexpr (sizeof(OutT) == 4) {
-        // Round 6: the results leave COALESCED.  A thread owns 16 consecutive elements, so stored from its registers every store instruction of a
-        // wave wrote 4 bytes into each of 64 different lines; through a (padded) tile in LDS a wave writes 256 contiguous bytes per instruction.
+        // The results leave COALESCED.  A thread owns 16 consecutive elements, so stored from its registers every store instruction of a
+        // wave would write 4 bytes into each of 64 different lines; through a (padded) tile in LDS a wave writes 256 contiguous bytes per instruction.
 #pragma unroll
         for (int k = 0; k < SCAN_ITEMS; ++k) {
             const uint32_t j = threadIdx.x * SCAN_ITEMS + k;
@@ -606,8 +606,8 @@ __global__ __launch_bounds__(NW * 64) void k_tile3(ReadsDev R, const uint32_t* _
             __syncthreads();
         }
     }
-    // the vote statistic: every vote went into exactly one counter of its lane, and the draft's own context opened c0 with 1 (round 6: it
-    // used to be counted vote by vote inside the record loop)
+    // the vote statistic: every vote went into exactly one counter of its lane, and the draft's own context opened c0 with 1 (counted
+    // here and not vote by vote inside the record loop)
     uint32_t tsum = vl.c0 + vl.c1;
     for (uint32_t e = 2; e < vl.n; ++e) tsum += L[(e - 2) * 64 + lane] & 0xffffu;
     uint32_t nvotes = tsum - 1u;
@@ -624,7 +624,7 @@ __global__ __launch_bounds__(NW * 64) void k_tile3(ReadsDev R, const uint32_t* _
 
 
 // ------------------------------------------------------------------------------------------------
-// k_tile9 (default since round 4; np1_tile9.h has the idea and the per-lane logic, shared with the host model).
+// k_tile9 (NP1_TILE=9; np1_tile9.h has the idea and the per-lane logic, shared with the host model).
 // A workgroup of NW waves stages the descriptors and packed bases of its candidate records like k_tile3 does; every wave owns
 // T9_CH vote chunks (248 slots), four slots per lane.
 //   record loop   wave-uniform over the staged records, the record's fields fetched one record ahead and moved to scalar registers;
@@ -1452,7 +1452,7 @@ int launch_tile9(hipStream_t st, const ReadsDev& R, const uint32_t* soff, const 
     return 0;
 }
 
-// ---- intra-contig tiling: which slots left the vote with one state (the chain restarts behind each of them), and
+// ---- intra-contig tiling (np1_tile.cpp): which slots left the vote with one state (the chain restarts behind each of them), and
 // what a tile needs to know to be joined: is there such a slot in each halo, and where do its own bases start / end in the output
 __global__ __launch_bounds__(256) void k_single_map(const uint16_t* __restrict__ slot_res, uint32_t S, uint8_t* __restrict__ single) {
     const uint32_t s = blockIdx.x * blockDim.x + threadIdx.x;

@@ -136,7 +136,7 @@ int np1_pipe_run_resident(np1_pipe* p, const Configure* cfg, int task, int passe
     std::mutex err_mu;
     const size_t nl = p->lanes.size();
     // (pass, batch) pairs are handed out through one counter: a lane whose thread the system refuses is simply not there, and the
-    // lanes that did start take its share (round 3 strode the batches by lane index, which left every nl-th batch undone in that case)
+    // lanes that did start take its share (dealt by lane index, every nl-th batch would stay undone in that case)
     const size_t nb = p->resident.size();
     const size_t n_items = nb * (size_t)(passes > 0 ? passes : 0);
     std::atomic<size_t> next(0);
@@ -403,8 +403,8 @@ int np1_pipe_run_files(np1_pipe* p, const char* fasta, const char* bam, const ch
             cv.notify_all();          // (the emitter thread below hands the batches to the sink, in order)
         }
     };
-    // Round 6: the sink runs on a thread of its own.  It used to run on whichever lane finished a batch while nobody else was emitting -- and
-    // the CLI's sink writes the FASTA text into a pipe: 3 GB at the pace of the reader held one of three lanes half of the time.
+    // The sink runs on a thread of its own: the CLI's sink writes the FASTA text into a pipe, and on whichever lane had finished a batch, 3 GB at
+    // the pace of the reader held one of three lanes half of the time.
     auto emitter = [&]() {
         std::unique_lock<std::mutex> g(mu);
         for (;;) {

@@ -13,9 +13,9 @@
 struct np1_stream {
     np::ReadStream s;
     // np1_stream_pin: every array an upload moves (above the size the runtime stages itself) has a copy in ONE page-locked arena from
-    // hipHostMalloc, and uploads read from there -- asynchronous at full PCIe rate.  (Rounds 2-4 registered the std::vector storage
-    // itself with hipHostRegister; round 5 found the GPU faulting on heap addresses and took the GPU off the heap: DESIGN.md section 12.)
-    std::atomic<bool> pinned{false};      // set (release) once the arena and its map are complete, read (acquire) by every upload: ADVICE r5
+    // hipHostMalloc, and uploads read from there -- asynchronous at full PCIe rate.  (The std::vector storage itself is
+    // never registered: the GPU was seen to fault on heap addresses, np_hostcopy.h.)
+    std::atomic<bool> pinned{false};      // set (release) once the arena and its map are complete, read (acquire) by every upload
     std::mutex pin_mu;                    // one np1_stream_pin / np1_stream_unpin at a time
     void* arena = nullptr;
     size_t arena_bytes = 0;

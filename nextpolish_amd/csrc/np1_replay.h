@@ -6,7 +6,7 @@
 // the record behind the first chunk of the current chunk list re-uses that list -- made for another region -- and resumes at a saved
 // offset; the scan can then run out of chunks before it meets a record that starts behind the part, and the record left in the
 // buffer (which the level-1 fallback of kmercount.c:212-217 parses) is not "the next record in file order".  On drafts covered a
-// few times this changes a few bases per contig (DESIGN.md section 3).  Everything here is a function of record positions, end
+// few times this changes a few bases per contig.  Everything here is a function of record positions, end
 // positions, virtual offsets and the index -- not of the votes -- except which parts run the second loop.
 #pragma once
 #include <algorithm>

@@ -1,4 +1,4 @@
-// Intra-contig tiling of score_chain in the product (DESIGN.md section 8; the scheme and its proof by fuzz: tests/model/np1_model.cpp,
+// Intra-contig tiling of score_chain in the product (the scheme and its proof by fuzz: tests/model/np1_model.cpp,
 // np1m_score_chain_tiled).  A contig of any length -- the reference takes contigs up to 2^31 (source/nextPolish:101-102), one HBM
 // batch holds about 250 Mb at 30x -- is polished as independent tiles [a, b) with a halo on each side:
 //   * votes are local: a slot's pileup depends on the records that cover it (source/lib/contig.c:247-331), and
@@ -23,7 +23,7 @@
 #include "np_stream.h"
 
 // One contig opened for tiling: the FASTA index entry, the contig's draft and the BAM index are read ONCE and serve every tile of every
-// call (round 4 read all three again for every tile a rank asked for: O(tiles x contig length) of host I/O).
+// call (read again for every tile they would be O(tiles x contig length) of host I/O).
 struct np1_tiler {
     std::string fasta, bam, name;
     std::string draft;
@@ -93,10 +93,8 @@ int np1_tiler_run(np1_tiler* t, np1_ctx* ctx, const Configure* cfg, int64_t tile
     bool next_ready = false;
     std::thread loader;
     // While the device runs tile t a helper thread reads tile t + 1 (NP1_TILE_PREFETCH=0 switches that off: read, upload, run, release, tile
-    // after tile on one thread).  History: round 5 had this and a reused batch object as defaults for a day, then switched both off on suspicion
-    // after a one-process run of the GPU suite stopped inside a tiling test.  Round 6 found the stop: hipFree itself, in any long-lived process
-    //  -- the read-ahead thread makes no HIP call at all.  Since the allocator cache of np_devalloc.h a fresh batch per
-    // tile costs no runtime call in steady state, so the reused batch object is gone and the read-ahead is the default again.
+    // after tile on one thread).  The helper makes no HIP call at all.  With the allocator cache of np_devalloc.h a fresh batch per tile costs no
+    // runtime call in steady state, so no batch object is kept from tile to tile.
     static const bool prefetch = !(getenv("NP1_TILE_PREFETCH") && strcmp(getenv("NP1_TILE_PREFETCH"), "0") == 0);
     auto start_load = [&](size_t k) {
         next_ready = false;

@@ -1,4 +1,4 @@
-// k_tile9 (round 4): the pileup vote with FOUR SLOTS PER LANE and the agreeing votes counted per record, not per vote.
+// k_tile9: the pileup vote with FOUR SLOTS PER LANE and the agreeing votes counted per record, not per vote.
 //
 // What the reference does per vote (source/lib/contig.c:247-331, base.c:60-71) -- look the 3-base context up in the slot's list, bump
 // its count -- k_tile3 does per (record, 64-slot chunk) step with one lane per slot: ~75 vector instructions for 64 votes of which

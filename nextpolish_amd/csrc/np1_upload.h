@@ -1,4 +1,4 @@
-// The forms a record stream crosses PCIe in (DESIGN.md section 4): built once per stream on the host, undone on the device by the
+// The forms a record stream crosses PCIe in: built once per stream on the host, undone on the device by the
 // small kernels of np1_kernels.hip (k_unpack_seq2, k_unpack_draft4, k_patch_seq, k_expand_*).  Plain host code, no HIP: the product
 // calls the builders from np1_device.hip:stream_facts, and the CPU test-suite runs them against the host restatements of the undo
 // kernels at the end of this file (tests/model: np1m_upload_roundtrip) -- what comes back must be the stream's own arrays.

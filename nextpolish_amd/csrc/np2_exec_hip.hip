@@ -878,8 +878,8 @@ __global__ void k2_extract(const SubReqDev* rq, uint32_t n, const uint32_t* pre,
 
 // read coordinate of a stream at a window column (Exec::read_coords): a lane per request walks its stream's tag nibbles from the front --
 // eight at a time while the column lies beyond the word -- counting the tags that carry a base; the column's own tag is its need-th
-// non-insertion tag.  A few hundred requests per window with split reads; replaces the download of every tag stream of the window
-// (~40 MB) that the host walk needed (round 5).
+// non-insertion tag.  A few hundred requests per window with split reads; saves the download of every tag stream of the window
+// (~40 MB) that a walk on the host would need.
 struct CoordReqDev { uint32_t stream, col, through_col, pad; };
 __global__ void k2_read_coord(const CoordReqDev* rq, uint32_t n, const uint64_t* tag_off, const uint32_t* aln_t_s, const uint8_t* tags, uint32_t* out) {
     const uint32_t i = blockIdx.x * blockDim.x + threadIdx.x;
@@ -1696,8 +1696,8 @@ __global__ void k2_bt_place(const BtWalk* walks, uint32_t n_runs, const BtGroupP
 
 
 // ---- pseudo-seeds of the low-quality regions: one resident wave per job slot (np2_poa_dev.h) --------------------------------
-// A launch works through a list of job numbers (`order`, longest first) that its waves take off ONE atomic counter (round 4 dealt jobs in a
-// fixed stride: the slot that drew the long regions finished last with the others idle).  Three launches per window: the Small class (graph
+// A launch works through a list of job numbers (`order`, longest first) that its waves take off ONE atomic counter (dealt in a
+// fixed stride, the slot that drew the long regions finished last with the others idle).  Three launches per window: the Small class (graph
 // indices in bytes, score table in LDS, 9 waves a CU) on the jobs the host expects to fit it, at the same time the Big class (table in HBM
 // scratch, the last two rows in LDS) on the rest, then the Big class again on what the Small one gave back (redo_only: status 1); what Big
 // gives back goes to the host version.

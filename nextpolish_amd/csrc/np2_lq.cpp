@@ -90,7 +90,7 @@ struct Ranker {
     }
 
     // k-mer support of every candidate in play; `tail` selects the window.  Occurrences are counted in a small open-addressing table
-    // (<= 60 voters x 32 codes in 4096 slots; round 3 sorted the codes and searched them: ten times the work for the same counts).
+    // (<= 60 voters x 32 codes in 4096 slots; sorting the codes and searching them was ten times the work for the same counts).
     void add_support(bool tail, std::vector<uint32_t>* total) {
         constexpr uint32_t SLOTS = 4096, EMPTY = 0xffffffffu;
         static thread_local std::vector<uint32_t> key, cnt;          // key = the 16-bit code, or EMPTY

@@ -9,7 +9,7 @@
 //
 // Low-quality regions go through np2_lq.cpp (candidates, POA pseudo-seed, O(ND) alignment on the host; the graph
 // consensus of the concatenated regions in the executor).
-// The split-read structural layer (depth track, gap clusters, supplementary streams, split points) is in np2_sv.cpp.  See DESIGN.md section "path B".
+// The split-read structural layer (depth track, gap clusters, supplementary streams, split points) is in np2_sv.cpp.
 #include <algorithm>
 #include <cassert>
 #include <cctype>
@@ -854,7 +854,7 @@ static consensus_trimed_data* ctg_cns_core_task(ctg_cns_cfg* cfg, ref_* ref, cha
             if (getenv("NP2_SV_LOG")) { FILE* lg2 = fopen(getenv("NP2_SV_LOG"), "a"); if (lg2) { fprintf(lg2, "update_align_tags streams %u -> %u\n", sc0, seq_count); fclose(lg2); } }
         }
         lap("keep rules + structural");
-        in.want_tags = false;           // (round 5: generate_gapseqs asks the executor for the read coordinates it needs instead of walking the streams here)
+        in.want_tags = false;           // (generate_gapseqs asks the executor for the read coordinates it needs instead of walking the streams here)
         in.lq_ratio1 = reads_type == np2k::READS_HIFI ? 0.f : gap_min_ratio1;   // the executor marks where the low-quality scans have to look (NP2_LQ_TRIGGERS=0: off)
         if (!cfg->exec->run_window(in, &out, &err)) np2_die(err.c_str(), ref->n);
         lap("window (executor)");

@@ -24,7 +24,7 @@ namespace np2poa {
 
 constexpr int32_t W_MATCH = 1, W_MISMATCH = -2, W_GAP = -2;
 
-// Two size classes of one algorithm (round 5).  A job = the best six candidates of a region at most (np2_lq.cpp: rank_and_seed), typically
+// Two size classes of one algorithm.  A job = the best six candidates of a region at most (np2_lq.cpp: rank_and_seed), typically
 // 35-45 characters each, so its graph has a few dozen nodes and its score table a few thousand cells:
 //   Small  indices in one byte (127 nodes, 254 edges, strings up to 126 characters, 8 strings), the SCORE TABLE IN LDS as 16-bit scores +
 //          16-bit back pointers (3072 cells): 16.9 KB of LDS a wave, 9 regions a CU, and a row of the table costs LDS round trips where the
@@ -226,7 +226,7 @@ template <class C> __device__ void add_string(Graph<C>& G, uint32_t q, const cha
         const uint32_t R0 = row * width;
         const uint32_t e0 = uni(L->in_head[v]);
         // The rows this row reads (its predecessors' rows; a source reads row 0), found ONCE per row and kept in scalars -- the border,
-        // the "anything but the row just made?" test and every 64-column chunk below go over them (round 5: each of those walked the edge
+        // the "anything but the row just made?" test and every 64-column chunk below go over them (instead of each walking the edge
         // list through LDS again, three dependent reads per edge and chunk).  More than four predecessors: the walk is repeated as before.
         uint32_t p0 = 0, p1 = 0, p2 = 0, p3 = 0, n_pred = 0;
         if (e0 == NONE16) { n_pred = 1; }

@@ -288,7 +288,7 @@ namespace {
 // One cluster's search for the draft interval its split reads bridge, and the piece of every read that lies across it.  The search is
 // a small state machine so that ALL clusters of a window advance together: what needs the tag streams -- "which base of its read has
 // stream s reached at column c" -- is asked of the executor for every cluster at once (Exec::read_coords, a lane per question on the
-// device; round 4 downloaded every tag stream of the window, ~40 MB, and walked them here).
+// device; walked here, every tag stream of the window, ~40 MB, would have to be downloaded).
 struct GapBridge {
     SvWindow* w;
     SvCluster& clu;

@@ -535,8 +535,8 @@ int Fai::find(const std::string& name) const {
 // Whole sequence, printable characters only (fai_fetch).  The index gives the line layout (line_bases characters in line_width bytes),
 // so line k of the record lands at output offset k * line_bases whatever thread copies it: the lines are dealt over the host threads,
 // each pread()s its byte range and copies line by line, checking that every byte it takes is printable (one vectorisable pass).  A
-// record whose lines are not what the index says (blanks inside a line, ragged lines) takes the byte-by-byte path, like round 3 did
-// for every contig at ~250 MB/s -- a second per 250 Mb contig on the staging thread of the from-files pipeline.
+// record whose lines are not what the index says (blanks inside a line, ragged lines) takes the byte-by-byte path, which does
+// ~250 MB/s -- a second per 250 Mb contig on the staging thread of the from-files pipeline.
 bool Fai::fetch(int i, std::string* out) const {
     if (i < 0 || i >= (int)entries_.size()) return false;
     const FaiEntry& e = entries_[i];
@@ -556,7 +556,7 @@ bool Fai::fetch(int i, std::string* out) const {
                     const int64_t f0 = e.offset + l0 * lw;
                     const int64_t last_len = std::min<int64_t>(lb, e.len - (l1 - 1) * lb);
                     // (a job that is not the contig's last one reads its last line WITH the terminator, so that every line but the contig's
-                    // last is checked to end where the index says -- round 4 left the last line of each 8 MiB job unchecked)
+                    // last is checked to end where the index says, the last line of each 8 MiB job too)
                     const bool more = l1 < n_lines;
                     const int64_t bytes = (l1 - 1 - l0) * lw + last_len + (more ? 1 : 0);
                     buf.resize((size_t)bytes);

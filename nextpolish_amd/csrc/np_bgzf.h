@@ -37,8 +37,7 @@ public:
 private:
     // Blocks are independent deflate streams, so the reader inflates a window of consecutive blocks at once on a few
     // threads (NP_IO_THREADS, default min(8, cores); threads live only inside fill_window: fork-safe) and serves
-    // read()/seek() from that window.  This is the "BGZF ingest" row of SURVEY.md section 8(f): inflate is ~60 % of
-    // the reference's wall time.
+    // read()/seek() from that window: inflate is ~60 % of the reference's wall time.
     struct WinBlock { uint64_t coff; uint32_t total, isize; size_t cpos, upos; };
     bool load_block();                 // make the block at file offset next_coff_ current
     bool fill_window(uint64_t coff);   // read + inflate the blocks starting at coff

@@ -143,7 +143,7 @@ namespace np {
 
 // Installs the device inflater for every BgzfReader of this process (call after the HIP device of the worker is chosen).
 // Opt-in (NP2_INFLATE=device): it takes 43 % of a worker's host CPU time away (0.160 -> 0.091 CPU-s per Mbp) but adds ~15 ms of
-// GPU time per 5 Mb window, and eight workers sharing one GPU are GPU-bound (DESIGN.md section 10), so the default keeps the host
+// GPU time per 5 Mb window, and eight workers sharing one GPU are GPU-bound, so the default keeps the host
 // threads.  NP2_INFLATE_WINDOW_MB = compressed bytes gathered per launch at most (default 48; sequential reads grow towards it).
 void bgzf_device_inflate_enable(int device) {
     const char* e = getenv("NP2_INFLATE");

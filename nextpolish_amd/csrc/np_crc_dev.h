@@ -38,8 +38,8 @@ inline void crc_shift_table(uint32_t* out) {
 
 // Four 256-entry tables into LDS by the first 256 threads of a workgroup (slicing by four: tab[k * 256 + b] = the CRC state a byte b
 // leaves k bytes further on).  Contains the barriers it needs; every thread of the workgroup has to call it.
-// Round 4: the byte-wise loop was one chain of dependent LDS lookups per byte (1 024 of them per lane and block, ~100 cycles each: the
-// kernel was bound by that latency, 7 % of the device time of the from-files pipeline); with four tables a word is four INDEPENDENT
+// A byte-wise loop is one chain of dependent LDS lookups per byte (1 024 of them per lane and block, ~100 cycles each: the
+// kernel was bound by that latency with it, 7 % of the device time of the from-files pipeline); with four tables a word is four INDEPENDENT
 // lookups, the chain is one lookup per word.
 __device__ __forceinline__ void crc_table_build(uint32_t* tab) {
     uint32_t c = 0;
@@ -73,7 +73,7 @@ __device__ __forceinline__ uint32_t crc_block_wave(const uint8_t* __restrict__ p
     };
     for (; i < hi && ((uintptr_t)(p + i) & 3u); ++i) c = tab[(c ^ p[i]) & 0xffu] ^ (c >> 8);
     for (; i + 4 <= hi && ((uintptr_t)(p + i) & 15u); i += 4) word(*reinterpret_cast<const uint32_t*>(p + i));
-    // 16 bytes per load (round 6): the lanes' pieces lie 1 KiB apart, so a load instruction touches 64 cache lines whatever its width --
+    // 16 bytes per load: the lanes' pieces lie 1 KiB apart, so a load instruction touches 64 cache lines whatever its width --
     // with one-word loads every line came in from L2 sixteen times (the 32 waves of a CU walk 2 MiB, far beyond its L1)
     for (; i + 16 <= hi; i += 16) {
         const uint4 v = *reinterpret_cast<const uint4*>(p + i);

@@ -19,7 +19,7 @@
 // NP_DEVPOISON=1 (debugging; or a hex byte, e.g. NP_DEVPOISON=ff): every new device buffer is filled with that byte (default a5) before it
 // is handed out.  hipMalloc hands a long-lived process the bytes of whatever it freed before -- a fresh process mostly sees zeros -- so a
 // kernel that reads memory nobody wrote behaves differently in the one-process test suite than in any single test; with the poison it
-// misbehaves the same way everywhere (DESIGN.md section 12).  NP_DEVPOISON=2 also fills the work buffers of a short-read batch before
+// misbehaves the same way everywhere.  NP_DEVPOISON=2 also fills the work buffers of a short-read batch before
 // every run (what an earlier run left in a reused buffer is the other thing only a long-lived process has).
 #pragma once
 #include <hip/hip_runtime.h>
@@ -42,11 +42,11 @@
 
 namespace npalloc {
 
-// NP_ALLOCLOG=<path> (debugging): every device allocation, pinned host allocation and host registration of both libraries, and every
-// release, is appended to <path>.<pid> as one line "<ms> <tid> <op> <address> <bytes>" (ops D+ D- device, H+ H- hipHostMalloc; round 5's hunt also logged R+ R- hipHostRegister,
-// which the libraries no longer use), written with one write(2) each so that the file is complete when the runtime ends the process on a GPU memory fault:
+// NP_ALLOCLOG=<path> (debugging): every device allocation and pinned host allocation of both libraries, and every
+// release, is appended to <path>.<pid> as one line "<ms> <tid> <op> <address> <bytes>" (ops D+ D- device, H+ H- hipHostMalloc),
+// written with one write(2) each so that the file is complete when the runtime ends the process on a GPU memory fault:
 // the address in the runtime's "Memory access fault by GPU ... on address" line is then looked up among the ranges that were live, or had
-// just been released, at that moment (tests/tools/r5_fault_lookup.py; DESIGN.md section 12).
+// just been released, at that moment (tests/tools/r5_fault_lookup.py).
 inline int alloc_log_fd() {
     static const int fd = [] {
         const char* e = getenv("NP_ALLOCLOG");
@@ -68,8 +68,8 @@ inline void alloc_log(const char* op, const void* p, size_t bytes) {
 }
 
 // Page-locked host memory of both libraries comes from here: hipHostMalloc, and a list of the ranges handed out -- np_hostcopy.h lets
-// the DMA engines touch host memory only when it lies in one of them (never the user's pageable pages, never a hipHostRegister of heap
-// memory: DESIGN.md section 12).
+// the DMA engines touch host memory only when it lies in one of them (never the user's pageable pages, never heap memory
+// registered with the runtime).
 struct PinnedRanges {
     std::mutex mu;
     std::map<uintptr_t, size_t> live;      // start -> bytes
@@ -84,7 +84,7 @@ inline bool is_pinned(const void* p, size_t bytes) {
     --it;
     return a >= it->first && a + bytes <= it->first + it->second;
 }
-// (round 6: pinned host memory goes through a BlockCache of its own, defined below -- hipHostFree waits for the device like hipFree does)
+// (pinned host memory goes through a BlockCache of its own, defined below -- hipHostFree waits for the device like hipFree does)
 inline hipError_t host_malloc(void** p, size_t bytes, unsigned flags);
 inline hipError_t host_free(void* p);
 

@@ -1,4 +1,4 @@
-// Abort diagnostics, off unless NP_ABORT_TRACE is set (tests/conftest.py sets it; DESIGN.md §12).
+// Abort diagnostics, off unless NP_ABORT_TRACE is set (tests/conftest.py sets it).
 //
 // A process that dies of SIGABRT inside native code says nothing about where: Python's faulthandler prints the Python frames, glibc and
 // libstdc++ print one line, the HIP runtime sometimes none.  With NP_ABORT_TRACE set, loading either library installs
@@ -41,7 +41,7 @@ void frames() {
     if (g_fd >= 0) backtrace_symbols_fd(pc, n, g_fd);
 }
 
-// Every other thread of the process prints its own native frames (round 6: a process that is ended from outside because it STOPPED -- the
+// Every other thread of the process prints its own native frames (a process that is ended from outside because it STOPPED -- the
 // test watchdog's SIGABRT to the blocked main thread, tests/conftest.py -- must say where each thread was: the runtime's own threads included).
 volatile sig_atomic_t g_thread_done = 0;
 
@@ -114,7 +114,7 @@ struct Install {
         const char* v = getenv("NP_ABORT_TRACE");
         if (!v || !*v || !strcmp(v, "0")) return;
         // the other library of the pair was first in THIS process (each holds its own copy of this unit).  The marker carries the pid: a
-        // child process inherits the environment and must still install its own handlers (ADVICE r4)
+        // child process inherits the environment and must still install its own handlers
         char me[32];
         snprintf(me, sizeof me, "%d", (int)getpid());
         const char* on = getenv("NP_ABORT_TRACE_ON");

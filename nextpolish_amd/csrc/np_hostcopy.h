@@ -1,6 +1,6 @@
 // Host <-> device copies of both libraries go through here.
 //
-// Why (round 5): on this runtime (ROCm 7.2) hipMemcpy / hipMemcpyAsync with PAGEABLE host memory is served three ways,
+// Why: on this runtime (ROCm 7.2) hipMemcpy / hipMemcpyAsync with PAGEABLE host memory is served three ways,
 // by size (its own log, AMD_LOG_LEVEL=4: profiles/r5_fault_hunt.txt section 2):
 //   <= 1 MiB          staged through the runtime's own pinned buffer: the bytes are taken (H2D) while the call runs;
 //   1 MiB .. 32 MiB   the USER's pages are locked in place ("Locking to pool", a userptr registration with the kernel driver), the DMA engine
@@ -35,7 +35,7 @@ namespace npcopy {
 
 constexpr size_t kDirectMax = 256 << 10;      // pageable copies up to this size are left to the runtime's own staging
 constexpr size_t kSlotBytes = 8 << 20;
-constexpr int kSlots = 16;      // (round 6: 6 -> 16: the from-files ingest reads half of them full in parallel while the other half is on its way to the device;
+constexpr int kSlots = 16;      // (more than 6: the from-files ingest reads half of them full in parallel while the other half is on its way to the device;
                                 // 32 x 4 MiB was measured too: no faster)
 
 struct Slot { void* p = nullptr; hipEvent_t ev = nullptr; bool pending = false; };
@@ -44,8 +44,8 @@ class Ring {      // one per device, library and slot size, made at the first pa
 public:
     Ring(size_t slot_bytes, int max_slots) : slot_bytes_(slot_bytes), max_slots_(max_slots) {}
     size_t slot_bytes() const { return slot_bytes_; }
-    // A slot to fill.  Blocks only while all kSlots exist and other threads hold them.  (Round 6: a new slot is allocated OUTSIDE the lock --
-    // hipHostMalloc can take milliseconds and used to stall every release() behind it; and a failed allocation only fails the call when
+    // A slot to fill.  Blocks only while all kSlots exist and other threads hold them.  (A new slot is allocated OUTSIDE the lock --
+    // hipHostMalloc can take milliseconds and would stall every release() behind it; and a failed allocation only fails the call when
     // there is no slot at all to wait for.)
     bool acquire(Slot* out) { return take(out, true); }
     // a slot only if one can be had without waiting for another thread to give one back (a thread that already holds a slot must not
@@ -102,7 +102,7 @@ private:
     bool alloc_failed_ = false;
 };
 
-constexpr size_t kSmallSlotBytes = kDirectMax;      // small pageable H2D copies (round 6): their own ring of small slots
+constexpr size_t kSmallSlotBytes = kDirectMax;      // small pageable H2D copies: their own ring of small slots
 constexpr int kSmallSlots = 32;
 struct Rings { std::mutex mu; std::map<int, Ring*> of; };      // (never destroyed: the runtime may already be gone when static destructors run)
 inline Rings& rings() { static Rings* r = new Rings(); return *r; }
@@ -127,7 +127,7 @@ inline hipError_t h2d(void* dst, const void* src, size_t bytes, hipStream_t q) {
     if (bytes <= kDirectMax) {
         // Small and pageable.  ROCm 7.2 stages such a copy through a pinned buffer of its own while the call runs -- but where "small" ends is
         // the runtime's business (and an environment variable's), and callers free the source as soon as this returns: the bytes go through a
-        // slot of ours, taken now (ADVICE r5).  Only without any pinned memory to be had is the copy left to the runtime, and waited for.
+        // slot of ours, taken now.  Only without any pinned memory to be had is the copy left to the runtime, and waited for.
         Ring& S = ring(true);
         Slot s;
         if (!S.acquire(&s)) {

@@ -1,5 +1,5 @@
 // Raw DEFLATE (RFC 1951) decoder for BGZF blocks, written from the RFC for this reader: BGZF inflate is the largest
-// single host cost of both polishing paths (SURVEY.md section 8f), and a decoder specialised for "whole block in, whole
+// single host cost of both polishing paths, and a decoder specialised for "whole block in, whole
 // block out" needs no stream state: 64-bit bit buffer refilled eight bytes at a time, one table lookup per symbol
 // (11-bit primary table for literals/lengths, 8-bit for distances, second-level tables for longer codes), the decoded
 // length known in advance.  Returns false on anything it does not accept (malformed or truncated input, output size
@@ -499,7 +499,7 @@ __attribute__((always_inline)) inline bool inflate_body(const uint8_t* src, size
 }
 
 bool inflate_plain(const uint8_t* src, size_t src_len, uint8_t* dst, size_t dst_len) { return inflate_body(src, src_len, dst, dst_len); }
-#if defined(__x86_64__)      // (the second build and its run-time dispatch exist on x86 only: ADVICE r4)
+#if defined(__x86_64__)      // (the second build and its run-time dispatch exist on x86 only)
 __attribute__((target("bmi,bmi2"))) bool inflate_bmi2(const uint8_t* src, size_t src_len, uint8_t* dst, size_t dst_len) { return inflate_body(src, src_len, dst, dst_len); }
 #endif
 

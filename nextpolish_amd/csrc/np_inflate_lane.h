@@ -28,7 +28,7 @@
 namespace nplane {
 
 constexpr int LIT_BITS = 10, DIST_BITS = 8;       // primary index bits.  (8 / 6 with a 16-bit copy of the primaries in LDS was measured: slower, 70 vs 98 GB/s --
-                                                  // three dependent loads for every code longer than the index cost more than the LDS lookups save; DESIGN.md 2b)
+                                                  // three dependent loads for every code longer than the index cost more than the LDS lookups save)
 constexpr uint32_t LIT_WORDS = (1u << LIT_BITS) + 1024u, DIST_WORDS = (1u << DIST_BITS) + 512u;   // primary + every possible second level
 constexpr uint32_t SUBBASE_WORDS = ((1u << LIT_BITS) + (1u << DIST_BITS)) / 2;   // 16-bit offsets of the second-level tables, one per possible head
 constexpr uint32_t SCRATCH_BYTES_EXTRA = 512 + (1u << LIT_BITS);     // code lengths + per-slot maxima while a table is built (bytes, behind the tables)

@@ -1,4 +1,4 @@
-// Raw DEFLATE (RFC 1951) decoder for whole BGZF blocks, ONE LANE PER BLOCK, written for a machine whose lanes run in lockstep (round 6).
+// Raw DEFLATE (RFC 1951) decoder for whole BGZF blocks, ONE LANE PER BLOCK, written for a machine whose lanes run in lockstep.
 //
 // np_inflate_lane.h is a sequential decoder per lane: tables in a 12 KB slice of HBM per lane, one load per table lookup and refill, every
 // match copied at once.  Measured (profiles/r6_inflate_lds.txt): with 40 000 blocks per launch a launch takes as long as ONE lane needs for
@@ -48,8 +48,8 @@ struct Scratch {
 // 16-bit slots of a lane's table.  Per alphabet: 2^bits primaries (symbol << 4 | code length, 0 = no code this short); for every code
 // length above `bits` the exclusive upper bound of its codes (15-bit, left-justified, in the order the bits arrive), what to add to a code
 // to index the symbols sorted by code, and (literal/length alphabet) the index in that order from which the symbols of this length are
-// >= 256; and ALL symbols sorted by code, their low eight bits, two to a slot.  (Round 6, third version: only the first 64 long symbols were
-// in LDS, the rest in HBM scratch -- and with 64 lanes in lockstep some lane needed one of the rest in most iterations, a trip to HBM for
+// >= 256; and ALL symbols sorted by code, their low eight bits, two to a slot.  (With only the first 64 long symbols
+// in LDS, the rest in HBM scratch, with 64 lanes in lockstep some lane needed one of the rest in most iterations, a trip to HBM for
 // the whole wave.  The symbol loop now reads nothing but LDS.)
 template <int LB, int DB> struct Layout {
     static constexpr uint32_t NL = 15 - LB, ND = 15 - DB;

@@ -47,7 +47,7 @@ bool load_stream(const std::string& fasta, const std::string& bam, const std::ve
     BamReader rd;
     if (!rd.open(bam)) { *err = "cannot open BAM: " + bam; return false; }
     // records could be used in place inside the BGZF window (every record is consumed before the next one is read), but
-    // on the GPU box's host the copying reader is ~10 % faster end to end (the copy doubles as a prefetch): opt-in only
+    // on the 16 cores it was measured on the copying reader is ~10 % faster end to end (the copy doubles as a prefetch): opt-in only
     rd.set_zero_copy(getenv("NP_BAM_ZERO_COPY") != nullptr);
     const BamHeader& hdr = rd.header();
 

@@ -6,7 +6,7 @@
 // (reference: source/lib/contig.c:202-358,632-686 read core.pos/flag/n_cigar/l_qseq/isize/qual,
 // the CIGAR array, the 4-bit sequence and, for kmer_count, the base qualities
 // source/lib/kmercount.c:365-465).  Algorithmic bytes per record = 32 (fixed fields below)
-// + 4*n_cigar + ceil(l_qseq/2) [+ l_qseq with qualities]  (SURVEY.md §8d).
+// + 4*n_cigar + ceil(l_qseq/2) [+ l_qseq with qualities].
 #pragma once
 #include <cstdint>
 #include <string>
@@ -46,7 +46,7 @@ struct ReadStream {
     size_t n_reads() const { return pos.size(); }
     size_t n_contigs() const { return names.size(); }
     void clear();
-    // bytes the roofline accounting uses (SURVEY.md §8d): records + draft (+ quals)
+    // bytes the roofline accounting uses: records + draft (+ quals)
     uint64_t algorithmic_input_bytes(bool with_qual) const;
 };
 
@@ -59,7 +59,7 @@ bool load_stream(const std::string& fasta, const std::string& bam, const std::ve
 // Mean-insert-size probe of config_init (reference: source/lib/config.c:80-101): scans the first
 // records of the BAM; returns sum/count with count starting at 1, and the first qualifying l_qseq.
 struct BaiIndex;
-// One TILE of one contig (intra-contig tiling): the records of `name` that touch draft bases [e_lo, e_hi] -- as the
+// One TILE of one contig (intra-contig tiling, np1_tile.cpp): the records of `name` that touch draft bases [e_lo, e_hi] -- as the
 // reference's walk sees them: a record ends where its M and D operations end, contig.c:262-326 -- read through the index, in file order, as
 // a stream of ONE contig whose draft is the hull [*lo, *hi) of those records and of the interval itself, widened by one base on each side
 // (position 0 and the last base of a contig are special to the walk, and no record of the tile may meet an artificial one).  Record

@@ -598,7 +598,7 @@ bool synth_stream_on(const np_synth_params& p, const std::vector<std::string>& n
     return true;
 }
 
-// Long-read workload of the nextpolish2 path (BASELINE configs[3]): a random draft per contig and noisy reads with
+// Long-read workload of the nextpolish2 path: a random draft per contig and noisy reads with
 // log-normal lengths whose CIGAR against the draft follows from the error process (substitution / insertion /
 // deletion per draft base, indel lengths uniform in 1..max_indel, first and last column always a match, optional
 // soft clips).  Reads come out sorted by position.

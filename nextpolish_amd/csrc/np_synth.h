@@ -1,4 +1,4 @@
-// Synthetic polishing workload generator (SURVEY.md §8d "synthetic inputs"): a truth genome, a
+// Synthetic polishing workload generator: a truth genome, a
 // draft assembly derived from it by long-read-assembly-like edits, and paired-end short reads
 // sampled from the truth whose CIGARs against the *draft* follow from the known edit script.
 // Output is a decoded ReadStream (for the HBM-resident benchmark) that can also be serialised as

@@ -215,7 +215,7 @@ def score_chain_tiled(ctx, fasta, bam, name, cfg, tile_bp, halo_bp):
     return seq
 
 
-# ---- the tiles of one dominant contig over the ranks of a node (--world > 1 with --tile_bp; DESIGN.md section 8) ------------------------
+# ---- the tiles of one dominant contig over the ranks of a node (--world > 1 with --tile_bp) ------------------------
 # Tiles are independent (np1_tile.cpp), so rank r polishes tiles r, r + world, ... of every contig longer than --tile_bp and leaves each
 # piece as a file in --tile_dir (a directory all ranks see); the contig's joiner -- rank (its position among such contigs) mod world --
 # concatenates the pieces in tile order and writes the record into its own -o part.  No collective, no process group: files, written
@@ -270,7 +270,7 @@ def device_tile_pieces(ctx, fasta, bam, cfg, tile_bp, halo_bp):
 def tile_run_token(genome, bam, cfg, tile_bp, halo_bp, world, launch_id=""):
     """what the pieces of one launch have in common and the leftovers of another launch have not: the input files as they are now (size,
     mtime), every parameter of the task and the tiling.  Pieces carry it in their first line; the joiner takes no piece without it (a
-    directory left by a killed run on other inputs or parameters is not stitched into this run's output: ADVICE r4)."""
+    directory left by a killed run on other inputs or parameters is not stitched into this run's output)."""
     import hashlib
     h = hashlib.md5()
     for path in (genome, bam):
@@ -282,7 +282,7 @@ def tile_run_token(genome, bam, cfg, tile_bp, halo_bp, world, launch_id=""):
         if isinstance(v, (int, float)):
             h.update(("%s=%r;" % (f, v)).encode())
     h.update(("%d:%d:%d" % (tile_bp, halo_bp, world)).encode())
-    # --launch_id: what the ranks of ONE launch share and a re-run of the same command does not (ADVICE r5: the token above is a pure function
+    # --launch_id: what the ranks of ONE launch share and a re-run of the same command does not (the token above is a pure function
     # of inputs and parameters, so a rank of the re-run that reaches the join before its slower peer has restarted would take the peer's
     # FAILED marker -- or a piece -- of the failed launch for this launch's)
     h.update(("|" + str(launch_id)).encode())

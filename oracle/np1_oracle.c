@@ -3,8 +3,8 @@
  * CPU restatement of nextpolish1.so's score_chain and kmer_count on a decoded record
  * stream.  Every routine cites the reference lines it restates; data structures mirror
  * the reference's per-base lists so that first-seen ordering, uint16 counters and the
- * traversal quirks fall out naturally.  Written from the behaviour described in
- * SURVEY.md appendix A/A2 and checked against the compiled reference (oracle/_ref).
+ * traversal quirks fall out naturally.  Written from the reference's behaviour
+ * and checked against the compiled reference (oracle/_ref).
  */
 #include "np1_oracle.h"
 

@@ -108,3 +108,11 @@ def test_hip_sources_are_compiled_without_packed_fp32():
     assert re.search(r"\$\(HIPCC\) \$\(HIPFLAGS\) -c", text) and len(re.findall(r"\$\(HIPCC\)[^\n]* -c ", text)) == 1
     bad = [path for path, body in texts() if path.startswith("nextpolish_amd") and re.search(r"v_pk_(add|mul|fma)_f32", body)]
     assert not bad, bad
+
+
+def test_the_sources_stand_on_their_own():
+    # what a comment says can be read without the documents beside the tree
+    away = re.compile(r"\b[A-Z]{5,}\.md\b|§|\b[A-Z]{6,} r\d\b|\b[Rr]ound[s-]? ?[3-9]\b")
+    bad = ["%s:%d" % (path, k) for path, text in texts() if path.startswith(("nextpolish_amd", "include", "oracle", "bench.py", "pytest.ini"))
+           for k, line in enumerate(text.splitlines(), 1) if away.search(re.sub(r"SAMv1 §[\d., §]+", "", line))]
+    assert not bad, bad
